@@ -41,6 +41,15 @@ class KVPoolSpec:
             pool[s:e].copy_(torch.randn((e - s, elems), generator=g, dtype=torch.float32))
         return pool.view(torch.uint8).view(pages, self.page_bytes)
 
+    def as_cache(self, pool: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """The [pages, 2, kv_heads, page_tokens, head_dim] cache that a [pages, page_bytes] uint8 pool (or pages of
+        one, gathered into HBM) holds: the same memory, keys before values in each page."""
+        if pool.dim() != 2 or pool.dtype != torch.uint8 or pool.shape[1] != self.page_bytes:
+            raise ValueError(f"expected a [pages, {self.page_bytes}] uint8 pool")
+        if torch.empty((), dtype=dtype).element_size() != self.dtype_bytes:
+            raise ValueError(f"{dtype} is not {self.dtype_bytes} bytes wide")
+        return pool.view(dtype).view(pool.shape[0], 2, self.kv_heads, self.page_tokens, self.head_dim)
+
     def sample_pages(self, pages: int, n: int, seed: int) -> torch.Tensor:
         """n page indices drawn uniformly without replacement."""
         g = torch.Generator().manual_seed(seed)

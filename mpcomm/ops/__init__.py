@@ -14,6 +14,10 @@ a host without the native module or a GPU these functions raise.
                                           (NVLS multimem or P2P bulk stores)
   nvls_broadcast(src, mc_ptr)             multimem.st broadcast
   p2p_fanout(src, dst_ptrs)               store the same bytes to peers
+  rotary(x, positions, inv_freq)          rotary positions, with gradient
+  paged_append(k, v, pool, ...)           keys and values into a paged cache,
+                                          rotated on the way
+  paged_attention(q, pool, ...)           attention over a paged cache
 
 ``pool`` may be pinned host memory (page-locked CPU tensor: the GPU reads it
 over PCIe through UVA) or device memory.
@@ -25,13 +29,14 @@ from typing import Optional, Sequence
 import torch
 
 from .. import _native
+from .kv import paged_append, paged_attention, rotary, rotary_frequencies
 
 MODE_AUTO, MODE_SM, MODE_TMA = 0, 1, 2
 
 __all__ = [
     "MODE_AUTO", "MODE_SM", "MODE_TMA", "paged_gather", "paged_scatter", "crc32_blocks",
     "copy_spans", "pxn_gather_forward", "gather_bcast", "nvls_broadcast", "p2p_fanout", "wait_flag",
-    "crc32_host",
+    "crc32_host", "rotary_frequencies", "rotary", "paged_append", "paged_attention",
 ]
 
 

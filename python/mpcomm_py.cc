@@ -8,13 +8,16 @@
 
 #include <unistd.h>
 
+#include <array>
 #include <atomic>
 #include <chrono>
 #include <cstring>
+#include <optional>
 #include <string>
 #include <vector>
 
 #include "cuda/gpu.h"
+#include "kernels/kv.h"
 #include "kernels/launch.h"
 #include "mpcomm.h"
 #include "parallel/vmm.h"
@@ -25,6 +28,54 @@ namespace py = pybind11;
 using namespace mpcomm;
 
 namespace {
+
+// (table, is64, row stride, width, lens, is64, starts, is64, seqs, page_tokens, pages)
+using KvBatchTuple = std::array<int64_t, 11>;
+
+kern::IndexPtr index_ptr(int64_t p, int64_t is64) {
+    kern::IndexPtr i;
+    i.ptr = reinterpret_cast<const void *>(p);
+    i.is64 = static_cast<int>(is64);
+    return i;
+}
+
+kern::KvBatch kv_batch(const KvBatchTuple &t) {
+    kern::KvBatch b;
+    b.table = index_ptr(t[0], t[1]);
+    b.table_stride = t[2];
+    b.table_width = t[3];
+    b.lens = index_ptr(t[4], t[5]);
+    b.starts = index_ptr(t[6], t[7]);
+    b.seqs = static_cast<int>(t[8]);
+    b.page_tokens = static_cast<int>(t[9]);
+    b.pages = t[10];
+    return b;
+}
+
+// Bytes [first, second) that a group's source or destination spans.
+std::pair<uintptr_t, uintptr_t> kv_span(const kern::KvRowsArgs &a, const kern::KvRowGroup &g, bool dst, int size) {
+    const bool paged = dst && g.plane >= 0;
+    const int64_t tokens = paged ? a.batch.page_tokens : a.tokens;
+    const int64_t batch = paged ? a.batch.pages : a.rows / (a.tokens > 0 ? a.tokens : 1);
+    const int64_t last = (batch - 1) * (dst ? g.db : g.sb) + (tokens - 1) * (dst ? g.dt : g.st) +
+                         (g.heads - 1) * (dst ? g.dh : g.sh) + (a.dim - 1) * (dst ? g.dd : g.sd);
+    const auto base = reinterpret_cast<uintptr_t>(dst ? g.dst : g.src);
+    return {base, batch > 0 && tokens > 0 && g.heads > 0 ? base + (last + 1) * size : base};
+}
+
+// A destination is its own source or shares no memory with any source.
+void refuse_overlap(const kern::KvRowsArgs &a, int size) {
+    for (int i = 0; i < a.groups; ++i) {
+        const kern::KvRowGroup &d = a.group[i];
+        if (d.plane < 0 && d.src == d.dst && d.sb == d.db && d.st == d.dt && d.sh == d.dh && d.sd == d.dd) continue;
+        const auto to = kv_span(a, d, true, size);
+        for (int j = 0; j < a.groups; ++j) {
+            const auto from = kv_span(a, a.group[j], false, size);
+            if (to.first < from.second && from.first < to.second)
+                throw py::value_error("a destination overlaps a source that it is not");
+        }
+    }
+}
 
 class PyMPComm {
  public:
@@ -819,6 +870,91 @@ PYBIND11_MODULE(_mpcomm, m) {
         return vmm::multicast_teardown(mc, mem, reinterpret_cast<void *>(uc), reinterpret_cast<void *>(mcva), size,
                                        dev);
     });
+
+    // ---- paged KV cache operators ----
+    m.def(
+        "kv_rows",
+        [](const std::vector<std::array<int64_t, 13>> &groups, int dim, int pairs, bool interleaved, int64_t rows,
+           int64_t tokens, uintptr_t inv_freq, bool freq_f64, float magnitude, float sign, uintptr_t positions,
+           int pos64, int64_t pos_sb, int64_t pos_st, const std::optional<KvBatchTuple> &batch, int dtype, int device,
+           uintptr_t stream, uintptr_t status) {
+            kern::KvRowsArgs a;
+            if (groups.empty() || groups.size() > 3) throw py::value_error("kv_rows takes one to three groups");
+            for (const auto &g : groups) {
+                kern::KvRowGroup &q = a.group[a.groups++];
+                q.src = reinterpret_cast<const void *>(g[0]);
+                q.dst = reinterpret_cast<void *>(g[1]);
+                q.sb = g[2], q.st = g[3], q.sh = g[4], q.sd = g[5];
+                q.db = g[6], q.dt = g[7], q.dh = g[8], q.dd = g[9];
+                q.heads = static_cast<int>(g[10]);
+                q.rotate = static_cast<int>(g[11]);
+                q.plane = static_cast<int>(g[12]);
+                a.heads += q.heads;
+            }
+            a.dim = dim;
+            a.pairs = pairs;
+            a.interleaved = interleaved;
+            a.rows = rows;
+            a.tokens = tokens;
+            a.inv_freq = reinterpret_cast<const void *>(inv_freq);
+            a.freq_f64 = freq_f64;
+            a.magnitude = magnitude;
+            a.sign = sign;
+            a.positions = index_ptr(positions, pos64);
+            a.pos_sb = pos_sb;
+            a.pos_st = pos_st;
+            if (batch) {
+                a.in_batch = 1;
+                a.batch = kv_batch(*batch);
+            }
+            a.status = reinterpret_cast<uint32_t *>(status);
+            refuse_overlap(a, dtype == kern::kFp32 ? 4 : 2);
+            py::gil_scoped_release r;
+            return kern::kv_rows(a, dtype, device, reinterpret_cast<void *>(stream));
+        },
+        py::arg("groups"), py::arg("dim"), py::arg("pairs"), py::arg("interleaved"), py::arg("rows"),
+        py::arg("tokens"), py::arg("inv_freq"), py::arg("freq_f64"), py::arg("magnitude"), py::arg("sign"),
+        py::arg("positions"), py::arg("positions_i64"), py::arg("positions_sb"), py::arg("positions_st"),
+        py::arg("batch"), py::arg("dtype"), py::arg("device"), py::arg("stream"), py::arg("status") = 0,
+        "Rotates and copies rows of heads; each group is (src, dst, four source strides, four destination strides, "
+        "heads, rotate, cache plane or -1), batch the paged batch's description or None.");
+    m.def("paged_attention_workspace", &kern::paged_attention_workspace, py::arg("rows"), py::arg("q_heads"),
+          py::arg("kv_heads"), py::arg("dim"), py::arg("seqs"), py::arg("device"),
+          "Bytes of workspace that paged_attention needs (any contents, 16-byte aligned).");
+    m.def(
+        "paged_attention",
+        [](uintptr_t q, int64_t q_st, int64_t q_sh, uintptr_t out, int64_t o_st, int64_t o_sh, uintptr_t lse,
+           uintptr_t pool, int64_t pool_page, int64_t pool_plane, int64_t pool_head, int64_t pool_token, int64_t rows,
+           int q_heads, int kv_heads, int dim, float scale, bool causal, int64_t window, bool fill_tail,
+           const KvBatchTuple &batch, uintptr_t workspace, size_t workspace_bytes, int dtype, int device,
+           uintptr_t stream, uintptr_t status) {
+            kern::PagedAttentionArgs a;
+            a.q = reinterpret_cast<const void *>(q);
+            a.q_st = q_st, a.q_sh = q_sh;
+            a.out = reinterpret_cast<void *>(out);
+            a.o_st = o_st, a.o_sh = o_sh;
+            a.lse = reinterpret_cast<float *>(lse);
+            a.pool = reinterpret_cast<const void *>(pool);
+            a.pool_page = pool_page, a.pool_plane = pool_plane, a.pool_head = pool_head, a.pool_token = pool_token;
+            a.rows = rows;
+            a.q_heads = q_heads, a.kv_heads = kv_heads, a.dim = dim;
+            a.scale = scale;
+            a.causal = causal;
+            a.window = window;
+            a.fill_tail = fill_tail;
+            a.batch = kv_batch(batch);
+            a.workspace = reinterpret_cast<void *>(workspace);
+            a.workspace_bytes = workspace_bytes;
+            a.status = reinterpret_cast<uint32_t *>(status);
+            py::gil_scoped_release r;
+            return kern::paged_attention(a, dtype, device, reinterpret_cast<void *>(stream));
+        },
+        py::arg("q"), py::arg("q_st"), py::arg("q_sh"), py::arg("out"), py::arg("o_st"), py::arg("o_sh"),
+        py::arg("lse"), py::arg("pool"), py::arg("pool_page"), py::arg("pool_plane"), py::arg("pool_head"),
+        py::arg("pool_token"), py::arg("rows"), py::arg("q_heads"), py::arg("kv_heads"), py::arg("dim"),
+        py::arg("scale"), py::arg("causal"), py::arg("window"), py::arg("fill_tail"), py::arg("batch"),
+        py::arg("workspace"), py::arg("workspace_bytes"), py::arg("dtype"), py::arg("device"), py::arg("stream"),
+        py::arg("status") = 0);
 
     // ---- host-side fault hooks of the loopback fabric (tests) ----
     m.def("_lo_inject_wc_errors", &fabric::loopback_inject_wc_errors, py::arg("gid"), py::arg("count"));

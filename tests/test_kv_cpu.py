@@ -1,0 +1,149 @@
+"""Paged KV cache operators without a GPU: frequencies, cache views and every refusal."""
+import math
+
+import pytest
+import torch
+
+import kv_reference as ref
+from mpcomm import ops
+from mpcomm.models import LLAMA3_8B_KV, KVPoolSpec
+
+BF16 = torch.bfloat16
+
+
+def _refused(call, for_the_device=False):
+    with pytest.raises(ValueError) as e:
+        call()
+    assert ("runs on CUDA tensors" in str(e.value)) == for_the_device, str(e.value)
+
+
+def test_frequencies():
+    plain = ops.rotary_frequencies(8, 10000.0)
+    assert plain.dtype == torch.float64
+    assert torch.allclose(plain, torch.tensor([1.0, 0.1, 0.01, 0.001], dtype=torch.float64), rtol=1e-14)
+    assert torch.equal(ops.rotary_frequencies(8, scaling="linear", factor=4.0), plain / 4.0)
+    wide = ops.rotary_frequencies(8, scaling="base", factor=3.0)
+    assert wide[0] == 1.0 and math.isclose(wide[-1], plain[-1] / 3.0, rel_tol=1e-13)
+    n = 128
+    f = ops.rotary_frequencies(n, 500000.0)
+    bands = ops.rotary_frequencies(n, 500000.0, "bands", 8.0, 8192, low=1.0, high=4.0)
+    ramp = ops.rotary_frequencies(n, 500000.0, "ramp", 8.0, 8192, low=1.0, high=32.0)
+    index = lambda turns: n * math.log(8192 / (turns * 2 * math.pi)) / (2 * math.log(500000.0))  # noqa: E731
+    first, last = math.floor(index(32.0)), math.ceil(index(1.0))
+    for i in range(n // 2):
+        turns = 8192 * f[i].item() / (2 * math.pi)
+        keep = 1.0 if turns > 4.0 else 0.0 if turns < 1.0 else (turns - 1.0) / 3.0
+        assert math.isclose(bands[i], f[i] * (keep + (1 - keep) / 8.0), rel_tol=1e-12)
+        keep = 1.0 - min(1.0, max(0.0, (i - first) / (last - first)))
+        assert math.isclose(ramp[i], f[i] * (keep + (1 - keep) / 8.0), rel_tol=1e-12)
+
+
+@pytest.mark.parametrize("args", [(7,), (0,), (8, 0.5), (8, 1e4, "spline"), (8, 1e4, "linear", 0.0), (2, 1e4, "base", 2.0),
+                                  (8, 1e4, "bands", 2.0), (8, 1e4, "ramp", 2.0, 100, 4.0, 4.0)])
+def test_frequencies_refuse(args):
+    with pytest.raises(ValueError):
+        ops.rotary_frequencies(*args)
+
+
+def test_cache_view_of_a_byte_pool():
+    spec = KVPoolSpec(kv_heads=2, head_dim=8, page_tokens=4)
+    pool = torch.arange(3 * spec.page_bytes, dtype=torch.int64).to(torch.uint8).view(3, spec.page_bytes)
+    cache = spec.as_cache(pool)
+    assert cache.shape == (3, 2, 2, 4, 8) and cache.data_ptr() == pool.data_ptr()
+    cache[1, 1, 0, 2] = 1.0
+    at = spec.page_bytes // 2 + 2 * 8 * 2  # the values' half of the page, third token of the first head
+    assert torch.equal(pool[1, at:at + 16].view(BF16), torch.ones(8, dtype=BF16))
+    assert LLAMA3_8B_KV.as_cache(torch.zeros(1, 65536, dtype=torch.uint8)).shape == (1, 2, 8, 16, 128)
+    for bad, dtype in ((pool[0], BF16), (pool[:, :-2], BF16), (pool.view(torch.int8), BF16), (pool, torch.float32)):
+        with pytest.raises(ValueError):
+            spec.as_cache(bad, dtype)
+
+
+def test_rotary_refuses():
+    x, pos, freq = torch.zeros(4, 2, 16, dtype=BF16), torch.arange(4), ops.rotary_frequencies(16)
+    for bad in (lambda: ops.rotary(x[0], pos, freq), lambda: ops.rotary(x.double(), pos, freq),
+                lambda: ops.rotary(x, pos[:3], freq), lambda: ops.rotary(x, pos.float(), freq),
+                lambda: ops.rotary(x, pos, ops.rotary_frequencies(18)), lambda: ops.rotary(x, pos, freq[:0]),
+                lambda: ops.rotary(x, pos, freq.half()), lambda: ops.rotary(x, pos, freq[::2]),
+                lambda: ops.rotary(x, pos, freq, out=x[:, :1]), lambda: ops.rotary(x, pos, freq, out=x.float()),
+                lambda: ops.rotary(x, pos, freq, out=x[:1].expand(4, 2, 16)),
+                lambda: ops.rotary(x.float().requires_grad_(), pos, freq, out=x.float())):
+        _refused(bad)
+    for plain in (lambda: ops.rotary(x, pos, freq, out=torch.zeros_like(x)), lambda: ops.rotary(x, pos, freq),
+                  lambda: ops.rotary(x.clone().requires_grad_(), pos, freq)):
+        _refused(plain, for_the_device=True)
+    with pytest.raises(RuntimeError):
+        ops.rotary(x, pos, freq, out=torch.zeros_like(x).requires_grad_())
+
+
+def _call(op, **change):
+    table, lens, starts, pages = ref.batch([3, 1], [20, 9], 8)
+    a = {"q": torch.zeros(4, 4, 16, dtype=BF16), "k": torch.zeros(4, 2, 16, dtype=BF16), "v": torch.zeros(4, 2, 16, dtype=BF16),
+         "pool": torch.zeros(pages, 2, 2, 8, 16, dtype=BF16), "table": table, "lens": lens, "starts": starts}
+    how = {n: v for n, v in change.items() if n not in a}
+    a.update({n: v(a[n]) if callable(v) else v for n, v in change.items() if n in a})
+    batch = (a["pool"], a["table"], a["lens"], a["starts"])
+    if op == "append":
+        return ops.paged_append(a["k"], a["v"], *batch, **how)
+    return ops.paged_attention(a["q"], *batch, **how)
+
+
+BATCH = [
+    {"pool": lambda t: t[:, 0]}, {"pool": lambda t: t[:, :1]}, {"pool": lambda t: t.float()}, {"pool": lambda t: t[..., :0]},
+    {"table": lambda t: t[0]}, {"table": lambda t: t.float()}, {"table": lambda t: t.t().contiguous().t()},
+    {"lens": lambda t: t[:1]}, {"lens": lambda t: t.to(torch.int16)}, {"lens": lambda t: t[:1].expand(2)},
+    {"starts": lambda t: t[:2]}, {"starts": lambda t: t.double()},
+]
+
+
+@pytest.mark.parametrize("change", BATCH + [
+    {}, {"k": lambda t: t[:, :1]}, {"k": lambda t: t.half()}, {"k": lambda t: t[..., :8]}, {"v": lambda t: t[:3]},
+    {"v": lambda t: t[0]}, {"pool": lambda t: t[:1].expand(9, 2, 2, 8, 16)}, {"inv_freq": torch.ones(9)},
+    {"inv_freq": torch.ones(8, dtype=torch.int64)}, {"q": None}, {"positions": torch.arange(4)},
+    {"inv_freq": torch.ones(8), "positions": torch.arange(3)}, {"inv_freq": torch.ones(8), "positions": torch.ones(4)},
+    {"inv_freq": torch.ones(8), "q_out": torch.zeros(4, 4, 16, dtype=BF16)},
+])
+def test_append_refuses(change):
+    if "q" in change:  # queries without frequencies
+        kv = torch.zeros(1, 2, 16, dtype=BF16)
+        _refused(lambda: ops.paged_append(kv, kv, torch.zeros(1, 2, 2, 8, 16, dtype=BF16), *ref.batch([1], [1], 8)[:3], q=kv))
+        return
+    _refused(lambda: _call("append", **change), for_the_device=not change)
+
+
+@pytest.mark.parametrize("change", BATCH + [
+    {}, {"q": lambda t: t[:, :3]}, {"q": lambda t: t[:, :0]}, {"q": lambda t: t.half()}, {"q": lambda t: t[..., :8]},
+    {"q": lambda t: t[0]}, {"window": -1}, {"window": 4, "causal": False}, {"out": torch.zeros(4, 4, 16)},
+    {"out": torch.zeros(3, 4, 16, dtype=BF16)}, {"out": torch.zeros(1, 4, 16, dtype=BF16).expand(4, 4, 16)},
+    {"out": torch.zeros(4, 4, 32, dtype=BF16)[..., ::2]}, {"out": torch.zeros(4, 4, 20, dtype=BF16)[..., :16]},
+    {"q": lambda t: torch.zeros(4, 4, 20, dtype=BF16)[..., :16]}, {"q": lambda t: torch.zeros(4, 4, 17, dtype=BF16)[..., 1:]},
+    {"q": lambda t: torch.zeros(16, 4, 4, dtype=BF16).permute(1, 2, 0)},
+    {"pool": lambda t: torch.zeros(8, 2, 2, 8, 20, dtype=BF16)[..., :16]}, {"pool": lambda t: t[..., :12]},
+    {"pool": lambda t: t[:, :, :, :4]}, {"pool": lambda t: torch.zeros(8, 2, 2, 8, 136, dtype=BF16)},
+    {"pool": lambda t: torch.zeros(8, 2, 2, 16, 8, dtype=BF16).transpose(3, 4)},
+])
+def test_attention_refuses(change):
+    _refused(lambda: _call("attention", **change), for_the_device=not change)
+
+
+def test_no_silent_loss_of_gradients():
+    grad = lambda t: t.clone().requires_grad_()  # noqa: E731
+    for op, name in (("append", "k"), ("append", "v"), ("append", "pool"), ("attention", "q"), ("attention", "pool")):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            _call(op, **{name: grad})
+
+
+def test_overlapping_destinations_are_refused():
+    """The binding compares the memory that sources and destinations span before anything is launched."""
+    import mpcomm
+
+    rows, heads, dim = 4, 2, 8
+    strides = (0, heads * dim, dim, 1)
+    call = lambda src, dst: mpcomm._native.kv_rows(  # noqa: E731
+        [(src, dst, *strides, *strides, heads, 1, -1)], dim, 0, False, 0, rows, 0, False, 1.0, 1.0, 0, 0, 0, 0, None, 0, 0, 0)
+    assert call(4096, 4096) == 0  # no rows: nothing is launched
+    call = lambda src, dst: mpcomm._native.kv_rows(  # noqa: E731
+        [(src, dst, *strides, *strides, heads, 1, -1)], dim, 0, False, rows, rows, 0, False, 1.0, 1.0, 0, 0, 0, 0, None, 7, 0, 0)
+    for shift in (2, 64, 126, -126):
+        with pytest.raises(ValueError):
+            call(4096, 4096 + shift)
