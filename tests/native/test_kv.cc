@@ -1,0 +1,149 @@
+// Host tests of the paged cache's index arithmetic and of paged attention's
+// plan: every block of every tile is done by exactly one CTA, every key that
+// a row sees lies in its tile's blocks, and tables with anything in them give
+// nothing outside the rows and pages there are.
+#include <cstdio>
+#include <cstdlib>
+#include <map>
+#include <random>
+#include <tuple>
+#include <vector>
+
+#include "kernels/attention_plan.h"
+
+using namespace mpcomm::kern;
+
+static long g_checks = 0;
+#define CHECK(cond)                                                          \
+    do {                                                                     \
+        ++g_checks;                                                          \
+        if (!(cond)) {                                                       \
+            std::printf("FAILED %s:%d: %s\n", __FILE__, __LINE__, #cond);    \
+            std::exit(1);                                                    \
+        }                                                                    \
+    } while (0)
+
+static void test_places() {
+    std::vector<int32_t> starts{0, 3, 3, 10};
+    std::vector<int64_t> table{4, 99, -1, 7, 0, 2};
+    KvBatch k;
+    k.starts.ptr = starts.data();
+    k.table.ptr = table.data();
+    k.table.is64 = 1;
+    k.table_stride = 2;
+    k.table_width = 2;
+    k.pages = 8;
+    k.seqs = 3;
+    k.page_tokens = 5;
+    const int want[] = {0, 0, 0, 2, 2, 2, 2, 2, 2, 2, -1, -1};
+    for (int r = 0; r < 12; ++r) CHECK(sequence_of(k, r) == want[r]);
+    CHECK(page_of(k, 0, 0) == 4 && page_of(k, 0, 4) == 4 && page_of(k, 0, 5) == -1);  // 99 is no page
+    CHECK(page_of(k, 1, 0) == -1 && page_of(k, 1, 9) == 7 && page_of(k, 1, 10) == -1 && page_of(k, 2, -1) == -1);
+    CHECK(page_of(k, 2, int64_t{1} << 40) == -1);
+    k.seqs = 0;
+    CHECK(sequence_of(k, 0) == -1);
+    // tables that are not ascending still give a sequence there is, or none
+    std::mt19937 rng(1);
+    for (int t = 0; t < 200; ++t) {
+        for (auto &s : starts) s = static_cast<int32_t>(rng());
+        k.seqs = 3;
+        for (int r = 0; r < 20; ++r) {
+            const int b = sequence_of(k, r);
+            CHECK(b >= -1 && b < 3);
+        }
+    }
+}
+
+static void check_plan(const PlanShape &s, const std::vector<int64_t> &starts, const std::vector<int64_t> &lens, int ctas) {
+    const int seqs = static_cast<int>(lens.size());
+    std::vector<PlanSeq> q;
+    int64_t units = 0;
+    for (int b = 0; b < seqs; ++b) {
+        q.push_back(plan_seq(s, starts[b], starts[b + 1], lens[b]));
+        CHECK(q[b].q0 >= 0 && q[b].new_tokens >= 0 && q[b].q0 + q[b].new_tokens <= s.rows);
+        CHECK(q[b].end >= 0 && q[b].end <= s.tokens);
+        units += s.kv_heads * plan_head_units(s, q[b]);
+        for (int m = 0; m < q[b].tiles; ++m) {
+            const PlanTile t = plan_tile(s, q[b], m);
+            CHECK(t.rows > 0 && t.rows <= kTileRows && t.blocks > 0 && t.block0 >= 0);
+            CHECK(t.lo >= 0 && t.hi <= q[b].end && t.lo <= t.hi);
+            CHECK(t.block0 * kBlockKeys <= t.lo && (t.block0 + t.blocks) * kBlockKeys >= t.hi);
+            int lo = 1 << 30, hi = 0;
+            for (int r = 0; r < t.rows; ++r) {
+                const int at = q[b].first + (m * kTileRows + r) / s.group;
+                int to = q[b].end, from = 0;
+                if (s.causal && at + 1 < to) to = at + 1;
+                if (s.window && at + 1 - s.window > 0) from = at + 1 - s.window;
+                if (from < to) {
+                    lo = from < lo ? from : lo;
+                    hi = to > hi ? to : hi;
+                }
+            }
+            if (hi) CHECK(t.lo <= lo && t.hi >= hi);
+        }
+    }
+    const int64_t share = plan_share(units, ctas);
+    CHECK(share * ctas >= units);
+    std::map<std::tuple<int, int, int, int>, int> done;
+    for (int c = 0; c < ctas; ++c) {
+        int64_t begin = c * share, left = units - begin < share ? units - begin : share;
+        if (left <= 0) continue;
+        int b = 0;
+        int64_t head = 0;
+        for (;; ++b) {
+            head = plan_head_units(s, q[b]);
+            if (begin < s.kv_heads * head) break;
+            begin -= s.kv_heads * head;
+        }
+        PlanCursor cur;
+        cur.seek(s, q[b], head, begin);
+        while (left > 0) {
+            PlanRun run;
+            if (!cur.next(s, q[b], left, &run)) {
+                ++b;
+                CHECK(b < seqs);
+                cur = PlanCursor();
+                continue;
+            }
+            CHECK(run.from < run.to && run.to <= run.tile.blocks);
+            for (int i = run.from; i < run.to; ++i) ++done[{b, run.h, run.m, i}];
+            left -= run.to - run.from;
+        }
+    }
+    CHECK(static_cast<int64_t>(done.size()) == units);
+    for (const auto &d : done) CHECK(d.second == 1);
+}
+
+static void test_plan() {
+    std::mt19937 rng(7);
+    auto pick = [&](int lo, int hi) { return lo + static_cast<int>(rng() % (hi - lo + 1)); };
+    for (int t = 0; t < 400; ++t) {
+        PlanShape s;
+        s.group = pick(1, t % 5 ? 9 : 300);
+        s.kv_heads = pick(1, 4);
+        s.causal = t % 4 != 0;
+        s.window = s.causal && t % 3 == 0 ? pick(1, 700) : 0;
+        s.tokens = pick(0, 2000);
+        const int seqs = pick(1, 12);
+        std::vector<int64_t> starts{0}, lens;
+        for (int b = 0; b < seqs; ++b) {
+            const int n = t % 2 ? pick(0, 2) : pick(0, 300);
+            starts.push_back(starts.back() + n);
+            lens.push_back(pick(0, 2) ? n + pick(0, 1500) : pick(0, 50));
+        }
+        s.rows = static_cast<int>(starts.back()) + pick(0, 3);
+        if (t % 10 == 9) {  // anything in the tables
+            for (auto &v : starts) v = static_cast<int64_t>(rng() % 4000) - 2000;
+            for (auto &v : lens) v = static_cast<int64_t>(rng()) << pick(0, 31);
+            lens[0] = -lens[0];
+        }
+        check_plan(s, starts, lens, t % 7 ? 148 : pick(1, 20));
+    }
+}
+
+int main() {
+    test_places();
+    test_plan();
+    std::printf("ok: %ld checks\n", g_checks);
+    return 0;
+}

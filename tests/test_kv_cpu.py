@@ -1,5 +1,7 @@
 """Paged KV cache operators without a GPU: frequencies, cache views and every refusal."""
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -147,3 +149,11 @@ def test_overlapping_destinations_are_refused():
     for shift in (2, 64, 126, -126):
         with pytest.raises(ValueError):
             call(4096, 4096 + shift)
+
+
+def test_native_plan():
+    """Index arithmetic of the paged cache and the split of attention's work over CTAs, on the host."""
+    exe = os.path.join(os.path.dirname(os.path.abspath(__file__)), "native", "bin", "test_kv")
+    assert os.path.exists(exe), "native tests not built (run __graft_entry__.build())"
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
