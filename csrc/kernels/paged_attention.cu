@@ -16,10 +16,11 @@
 // end, so the loads never wait for one stream's softmax.
 //
 //   warps 0-3, 4-7  the softmax of stream 0, 1: a thread has a row
-//   warp 8          walks the plan, loads K and V blocks by TMA (a page, or
-//                   the part of one that lies in the block, a box)
+//   warp 8          walks the plan, loads K blocks by TMA (a page, or the
+//                   part of one that lies in the block, a box)
 //   warp 9          issues the matrix instructions
-//   warps 10, 11    load the queries
+//   warp 10         loads the queries
+//   warp 11         loads V blocks
 //
 // Weights are rounded to the cache's type for the second product; sums,
 // maxima, scores and outputs are 32-bit. m only moves when a score passes it
@@ -43,8 +44,8 @@ namespace kern {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kStreamRows = 128;
 constexpr int kRunSlots = 4;
+constexpr int kFewTiles = 4;  // of a sequence, that one lane counts
 constexpr int kMaskSlots = 16;  // blocks whose masks are kept: more than are ever in flight
 constexpr float kRescale = 8.f;
 
@@ -52,16 +53,17 @@ __device__ uint32_t g_attention_status;
 
 // What the plan's warp tells the others of a run.
 struct RunInfo {
-    int blocks;  // 0: no more runs
-    int pair;    // each stream its own rows; else both streams the same
-    int rows;    // of the tile
-    int r0;      // the tile's first row in its sequence
-    int q0;      // the sequence's first row of the query tensor
-    int h;       // key head
-    int key0;    // first key of the run's first block
-    int first;   // position of the sequence's first new token
-    int end;     // keys of the sequence
-    int part;    // -1: the run is the whole tile; else its slot in the workspace
+    int blocks;    // 0: no more runs
+    int tokens;    // of the tile
+    int t0;        // the tile's first token among its sequence's new ones
+    int q0;        // the sequence's first row of the query tensor
+    int part;      // of the query heads
+    int key0;      // first key of the run's first block
+    int lo, hi;    // keys that some row of the tile sees
+    int first;     // position of the sequence's first new token
+    int end;       // keys of the sequence
+    int seq;
+    int slot;      // -1: the run is the whole tile; else its slot in the workspace
 };
 
 template <int DP>
@@ -87,20 +89,51 @@ struct Control {
     uint32_t dead;  // a wait ran out: nothing is waited for any more
 };
 
-struct Part {  // a tile whose blocks several CTAs share, from its first CTA on
+struct Shared {  // a tile whose blocks several CTAs share, from its first CTA on
     int pieces;
-    int q0, r0, rows, h;
+    int q0, t0, tokens, part;
 };
 
-// Bytes of a workspace: the parts, then two slots a CTA of kTileRows rows each.
-__host__ __device__ constexpr size_t parts_bytes(int ctas) { return (sizeof(Part) * ctas + 255) / 256 * 256; }
-__host__ __device__ constexpr size_t slot_bytes(int dp) { return static_cast<size_t>(kTileRows) * (dp + 2) * 4; }
+// Bytes of a workspace: what is shared, then two slots a CTA of two streams' rows each.
+__host__ __device__ constexpr size_t shared_bytes(int ctas) { return (sizeof(Shared) * ctas + 255) / 256 * 256; }
+__host__ __device__ constexpr size_t slot_bytes(int dp) { return static_cast<size_t>(2 * kStreamRows) * (dp + 2) * 4; }
+
+// How the pool lies in memory for the TMA. (page, plane, key head) is one
+// index in units of the greatest stride that divides all three, so that a box
+// of whole rows has dimensions to spare for its order in shared memory: with
+// heads of 64 or 128 elements one box is (64 elements, 8 slots, halves,
+// groups of 8 slots) and lands as groups of 8 rows, half by half. Other heads
+// end inside 64 elements, where the TMA has to fill up with zeros: their
+// boxes are (64 elements, slots), each half by itself.
+struct PoolView {
+    int page, plane, head;  // strides of the index
+    int none;               // an index behind the pool: reads as zeros
+    int whole;              // a box has both halves
+    int group_bytes, half_bytes;  // in shared memory: distance of 8-row groups, of halves
+};
+
+// Division of 31-bit values by a constant: a multiplication.
+struct FastDiv {
+    uint32_t times = 0, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d) {
+        // 2^(31 + ceil(log2 d)) / d, rounded up, is at most 2^32 - 1 and exact for 31-bit dividends
+        while ((1ull << shift) < d) ++shift;
+        times = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * times) >> (31 + shift));
+    }
+};
 
 struct KernelArgs {
     PagedAttentionArgs a;
     PlanShape shape;
+    PoolView pool;
+    FastDiv page_tokens;
+    int group;         // query heads of a key head
     float scale_log2;  // |scale| * log2(e)
-    uint32_t negate;   // sign bits to flip in the queries: scale is negative
+    int negate;        // scale is negative
     int ctas;
     int box;  // tokens of a full box
     uint64_t budget;
@@ -124,13 +157,17 @@ struct Kernel {
 
     __device__ uint32_t *status() const { return g.a.status ? g.a.status : &g_attention_status; }
 
-    // Waits for a phase; gives up after the budget, and at once when any wait of the CTA has given up.
+    // Waits for a phase; gives up after the budget, and at once when any wait of the CTA has given up. A try itself
+    // waits for some microseconds, so the clock is read only after many.
     __device__ __noinline__ void wait_slow(uint64_t *bar, uint32_t parity) const {
         volatile uint32_t *dead = &c->dead;
-        const uint64_t t0 = globaltimer_ns();
-        for (;;) {
+        uint64_t t0 = 0;
+        for (uint32_t n = 1;; ++n) {
             if (mbar_try_wait(bar, parity) || *dead) return;
-            if (globaltimer_ns() - t0 > g.budget) {
+            if (n % 64) continue;
+            const uint64_t now = globaltimer_ns();
+            if (!t0) t0 = now;
+            if (now - t0 > g.budget) {
                 *dead = 1;
                 atomicOr(status(), kStatusLoadTimeout);
                 return;
@@ -157,84 +194,125 @@ struct Kernel {
         return r;
     }
 
-    // ---- warp 8: the plan, and K and V ----
-    __device__ void load_loop(const CUtensorMap *boxes, const CUtensorMap *lines) const {
+    // ---- warp 8: the plan, and K ----
+    __device__ void plan_loop(const CUtensorMap *boxes, const CUtensorMap *lines) const {
         const KvBatch &k = g.a.batch;
         const PlanShape &s = g.shape;
-        int64_t units = 0;
-        for (int b0 = 0; b0 < k.seqs; b0 += 32) {
-            const int b = b0 + lane;
-            if (b < k.seqs) units += s.kv_heads * plan_head_units(s, plan_seq(s, k.starts.at(b), k.starts.at(b + 1), k.lens.at(b)));
-        }
+        auto sequence = [&](int b) { return plan_seq(s, k.starts.at(b), k.starts.at(b + 1), k.lens.at(b)); };
+        // Units of a part of each lane's sequence. A sequence of many tiles is counted by the whole warp.
+        auto count = [&](int b) {
+            PlanSeq q;
+            if (b < k.seqs) q = sequence(b);
+            int64_t own = q.tiles <= kFewTiles ? plan_part_units(s, q) : 0;
+            for (uint32_t many = __ballot_sync(~0u, q.tiles > kFewTiles); many; many &= many - 1) {
+                const int l = __ffs(many) - 1;
+                PlanSeq o;
+                o.new_tokens = __shfl_sync(~0u, q.new_tokens, l);
+                o.first = __shfl_sync(~0u, q.first, l);
+                o.end = __shfl_sync(~0u, q.end, l);
+                o.tiles = __shfl_sync(~0u, q.tiles, l);
+                int64_t n = plan_part_units(s, o, lane, 32);
 #pragma unroll
-        for (int o = 16; o; o >>= 1) units += __shfl_xor_sync(~0u, units, o);
+                for (int i = 16; i; i >>= 1) n += __shfl_xor_sync(~0u, n, i);
+                if (lane == l) own = n;
+            }
+            return own;
+        };
+        auto scan = [&](int64_t n) {
+#pragma unroll
+            for (int i = 1; i < 32; i <<= 1) {
+                const int64_t up = __shfl_up_sync(~0u, n, i);
+                if (lane >= i) n += up;
+            }
+            return n;
+        };
+        // The ring's memory, which nothing is loaded into yet, keeps the counts of a batch of more than a warp.
+        int64_t *kept = reinterpret_cast<int64_t *>(smem + L::kKv);
+        constexpr int kKept = L::kStages * L::kTile / 8;
+        int64_t own = 0, units = 0;
+        for (int b0 = 0; b0 < k.seqs; b0 += 32) {
+            own = count(b0 + lane);
+            units += own;
+            if (k.seqs > 32 && b0 + lane < kKept) kept[b0 + lane] = own;
+        }
+        int64_t sum = scan(units);
+        units = __shfl_sync(~0u, sum, 31) * s.parts;
         const int64_t share = plan_share(units, g.ctas);
         int64_t at = blockIdx.x * share;
         int64_t left = units - at < share ? units - at : share;
-        Part *part = static_cast<Part *>(g.a.workspace) + blockIdx.x;
-        Part mine{0, 0, 0, 0, 0};
+        Shared mine{0, 0, 0, 0, 0};
         int n_run = 0;
-        int64_t n_kv = 0;
-        int n_block = 0;
+        int64_t n_block = 0;
         if (left > 0) {
             // the sequence that holds unit `at`
             int b = 0;
-            int64_t head = 0;
-            for (int b0 = 0; b0 < k.seqs; b0 += 32) {
-                int64_t own = 0, sum;
-                if (b0 + lane < k.seqs)
-                    own = plan_head_units(s, plan_seq(s, k.starts.at(b0 + lane), k.starts.at(b0 + lane + 1), k.lens.at(b0 + lane)));
-                sum = own * s.kv_heads;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int64_t up = __shfl_up_sync(~0u, sum, o);
-                    if (lane >= o) sum += up;
+            for (int b0 = 0;; b0 += 32) {
+                if (k.seqs > 32) {
+                    own = b0 + lane < kKept ? (b0 + lane < k.seqs ? kept[b0 + lane] : 0) : count(b0 + lane);
+                    sum = scan(own);
                 }
-                const uint32_t past = __ballot_sync(~0u, sum > at);
+                const uint32_t past = __ballot_sync(~0u, sum * s.parts > at);
                 if (past) {
                     const int i = __ffs(past) - 1;
                     b = b0 + i;
-                    head = __shfl_sync(~0u, own, i);
-                    at -= __shfl_sync(~0u, sum, i) - head * s.kv_heads;
+                    own = __shfl_sync(~0u, own, i);
+                    at -= (__shfl_sync(~0u, sum, i) - own) * s.parts;
+                    break;
+                }
+                at -= __shfl_sync(~0u, sum, 31) * s.parts;
+            }
+            fence_proxy_async_smem();
+            PlanSeq q = sequence(b);
+            PlanCursor cur;
+            cur.part = static_cast<int>(plan_div(at, own));
+            at -= cur.part * own;
+            for (;; cur.m += 32) {  // its tile
+                const int blocks = cur.m + lane < q.tiles ? plan_tile(s, q, cur.m + lane).blocks : 0;
+                sum = scan(blocks);
+                const uint32_t past = __ballot_sync(~0u, sum > at);
+                if (past || cur.m + 32 >= q.tiles) {
+                    const int i = past ? __ffs(past) - 1 : 0;
+                    cur.block = static_cast<int>(at - __shfl_sync(~0u, sum - blocks, i));
+                    cur.m += i;
                     break;
                 }
                 at -= __shfl_sync(~0u, sum, 31);
             }
-            PlanSeq q = plan_seq(s, k.starts.at(b), k.starts.at(b + 1), k.lens.at(b));
-            PlanCursor cur;
-            cur.seek(s, q, head, at);
             while (left > 0) {
                 PlanRun run;
                 if (!cur.next(s, q, left, &run)) {
-                    ++b;
-                    q = plan_seq(s, k.starts.at(b), k.starts.at(b + 1), k.lens.at(b));
+                    if (++b >= k.seqs) break;
+                    q = sequence(b);
                     cur = PlanCursor();
                     continue;
                 }
                 left -= run.to - run.from;
                 const bool whole = run.from == 0 && run.to == run.tile.blocks;
-                if (run.from == 0 && !whole) {
+                RunInfo r;
+                r.blocks = run.to - run.from;
+                r.tokens = run.tile.tokens;
+                r.t0 = run.m * 2 * s.tokens_stream;
+                r.q0 = q.q0;
+                r.part = run.part;
+                r.key0 = (run.tile.block0 + run.from) * kBlockKeys;
+                r.lo = run.tile.lo;
+                r.hi = run.tile.hi;
+                r.first = q.first;
+                r.end = q.end;
+                r.seq = b;
+                r.slot = whole ? -1 : run.from == 0 ? 1 : 0;
+                if (r.slot == 1) {
                     const int64_t rest = run.tile.blocks - run.to;
-                    mine = Part{static_cast<int>(1 + (rest + share - 1) / share), q.q0, run.m * kTileRows, run.tile.rows, run.h};
+                    mine = Shared{static_cast<int>(1 + plan_div(rest + share - 1, share)), r.q0, r.t0, r.tokens, r.part};
                 }
                 const int slot = n_run % kRunSlots;
                 wait(&c->run_empty[slot], ((n_run / kRunSlots) & 1) ^ 1);
                 if (lane == 0) {
-                    RunInfo &r = c->run[slot];
-                    r.blocks = run.to - run.from;
-                    r.pair = run.tile.rows > kStreamRows;
-                    r.rows = run.tile.rows;
-                    r.r0 = run.m * kTileRows;
-                    r.q0 = q.q0;
-                    r.h = run.h;
-                    r.key0 = (run.tile.block0 + run.from) * kBlockKeys;
-                    r.first = q.first;
-                    r.end = q.end;
-                    r.part = whole ? -1 : run.from == 0 ? 1 : 0;
+                    c->run[slot] = r;
                     mbar_arrive(&c->run_full[slot]);
                 }
                 ++n_run;
-                load_run(boxes, lines, b, run, n_kv, n_block);
+                if (!load_blocks<0>(boxes, lines, r, n_block)) break;
             }
         }
         const int slot = n_run % kRunSlots;
@@ -242,79 +320,104 @@ struct Kernel {
         if (lane == 0) {
             c->run[slot].blocks = 0;
             mbar_arrive(&c->run_full[slot]);
-            if (g.a.workspace) *part = mine;
+            static_cast<Shared *>(g.a.workspace)[blockIdx.x] = mine;
         }
-        // After a wait that ran out, loads may be in flight that nobody has
-        // waited for: shared memory stays ours until they have landed.
-        if (gave_up() && lane == 0) {
-            for (int64_t i = n_kv > L::kStages ? n_kv - L::kStages : 0; i < n_kv; ++i)
-                mbar_wait_bounded(&c->kv_full[i % L::kStages], (i / L::kStages) & 1, g.budget);
-        }
+        drain_loads(2 * n_block);
     }
 
-    __device__ __forceinline__ int page_at(int b, int key, int lo, int hi, bool *bad) const {
-        if (key >= hi || key + g.box <= lo) return static_cast<int>(g.a.batch.pages);  // nobody sees it: zeros
-        const int64_t page = page_of(g.a.batch, b, key);
-        *bad = page < 0;
-        return page < 0 ? static_cast<int>(g.a.batch.pages) : static_cast<int>(page);
+    // ---- warp 11: V ----
+    __device__ void value_loop(const CUtensorMap *boxes, const CUtensorMap *lines) const {
+        int n_run = 0;
+        int64_t n_block = 0;
+        for (;;) {
+            const RunInfo r = take_run(n_run);
+            if (!r.blocks || !load_blocks<1>(boxes, lines, r, n_block)) break;
+        }
+        drain_loads(2 * n_block + 1);
     }
 
-    __device__ void load_run(const CUtensorMap *boxes, const CUtensorMap *lines, int b, const PlanRun &run, int64_t &n_kv,
-                             int &n_block) const {
-        const int nbox = kBlockKeys / g.box;
+    // After a wait that ran out, loads may be in flight that nobody has waited
+    // for: shared memory stays ours until they have landed. `next`: the
+    // warp's next load.
+    __device__ void drain_loads(int64_t next) const {
+        if (!gave_up() || lane) return;
+        for (int64_t i = next - 2; i >= 0 && i >= next - 2 * L::kStages; i -= 2)
+            mbar_wait_bounded(&c->kv_full[i % L::kStages], (i / L::kStages) & 1, g.budget / 8);
+    }
+
+    // The index of the page of key `key` on, g.pool.none where nobody sees the box or there is no page.
+    __device__ __forceinline__ int place(const RunInfo &r, int head, int plane, int key, bool *bad) const {
+        if (key >= r.hi || key + g.box <= r.lo) return g.pool.none;
+        // key is below plan's end, so its column is in the table
+        const int64_t page = g.a.batch.table.at(r.seq * g.a.batch.table_stride + g.page_tokens.div(key));
+        *bad = page < 0 || page >= g.a.batch.pages;
+        return *bad ? g.pool.none : static_cast<int>(page) * g.pool.page + plane * g.pool.plane + head * g.pool.head;
+    }
+
+    // Loads the blocks of a run into the ring: K of block i is load 2 i, V is load 2 i + 1. False: a wait gave up.
+    template <int PLANE>
+    __device__ bool load_blocks(const CUtensorMap *boxes, const CUtensorMap *lines, const RunInfo &r, int64_t &n_block) const {
+        const int nbox = kBlockKeys / g.box, nhalf = g.pool.whole ? 1 : kHalves;
         const int half = lane / nbox, box = lane - half * nbox;  // up to 16 boxes in each half
-        const bool active = half < kHalves;
-        const int lo = run.tile.lo, hi = run.tile.hi, none = static_cast<int>(g.a.batch.pages);
-        int key = (run.tile.block0 + run.from) * kBlockKeys + box * g.box;
+        const bool active = half < nhalf;
+        const int head = r.part / (g.shape.parts / g.a.kv_heads), none = g.pool.none;
+        const uint32_t at = box * (g.box / 8) * g.pool.group_bytes + half * g.pool.half_bytes;
+        int key = r.key0 + box * g.box;
         bool bad = false;
-        int page = active ? page_at(b, key, lo, hi, &bad) : none;
-        for (int i = run.from; i < run.to; ++i) {
-            const int now = page, now_key = key;
+        int index = active ? place(r, head, PLANE, key, &bad) : none;
+        for (int i = 0; i < r.blocks; ++i, ++n_block) {
+            const int now = index, now_key = key;
             const uint32_t bads = __ballot_sync(~0u, active && half == 0 && bad);
-            if (bads && lane == 0) atomicOr(status(), kStatusBadIndex);
+            if (PLANE == 0 && bads && lane == 0) atomicOr(status(), kStatusBadIndex);
             key += kBlockKeys;
             bad = false;
-            if (i + 1 < run.to && active) page = page_at(b, key, lo, hi, &bad);  // in flight while the block is loaded
-            const int slot = now_key % g.a.batch.page_tokens;
-            for (int plane = 0; plane < 2; ++plane, ++n_kv) {
-                const int stage = static_cast<int>(n_kv % L::kStages);
-                wait(&c->kv_empty[stage], ((n_kv / L::kStages) & 1) ^ 1);
-                if (gave_up()) return;
-                char *tile = smem + L::kKv + stage * L::kTile + half * kHalfBytes + box * g.box * 128;
-                uint64_t *bar = &c->kv_full[stage];
-                if (lane == 0) {
-                    if (plane == 0) c->mask[n_block % kMaskSlots] = ~bads;
-                    mbar_arrive_expect_tx(bar, L::kTile);
-                }
+            if (i + 1 < r.blocks && active) index = place(r, head, PLANE, key, &bad);  // in flight while this block is loaded
+            const int slot = now_key - g.page_tokens.div(now_key) * g.a.batch.page_tokens;
+            const int64_t n = 2 * n_block + PLANE;
+            const int stage = static_cast<int>(n % L::kStages);
+            wait(&c->kv_empty[stage], ((n / L::kStages) & 1) ^ 1);
+            if (gave_up()) return false;
+            char *tile = smem + L::kKv + stage * L::kTile;
+            uint64_t *bar = &c->kv_full[stage];
+            if (lane == 0) {
+                if (PLANE == 0) c->mask[n_block % kMaskSlots] = ~bads;
+                mbar_arrive_expect_tx(bar, L::kTile);
+            }
+            __syncwarp();
+            if (g.a.batch.pages == 0) {
+                // no pool to read: the tile is zeroed in place of its loads
+                for (int e = lane; e < L::kTile / 16; e += 32) reinterpret_cast<uint4 *>(tile)[e] = make_uint4(0, 0, 0, 0);
+                fence_proxy_async_smem();
                 __syncwarp();
-                if (g.a.batch.pages == 0) {
-                    // no pool to read: the tile is zeroed in place of its loads
-                    for (int e = lane; e < L::kTile / 16; e += 32)
-                        reinterpret_cast<uint4 *>(smem + L::kKv + stage * L::kTile)[e] = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0)
-                        asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-                                     "r"(static_cast<uint32_t>(L::kTile))
-                                     : "memory");
-                    continue;
-                }
-                // A box of values that is seen in part goes row by row: the rows that nobody sees as zeros.
-                const bool cut = plane == 1 && active && now != none && (now_key < lo || now_key + g.box > hi);
-                if (active && !cut) tma_load_5d(tile, boxes, bar, half * 64, slot, run.h, plane, now);
+                if (lane == 0)
+                    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                                 "r"(static_cast<uint32_t>(L::kTile))
+                                 : "memory");
+                continue;
+            }
+            // A box of values that is seen in part goes row by row: the rows that nobody sees as zeros.
+            const bool cut = PLANE == 1 && active && now != none && (now_key < r.lo || now_key + g.box > r.hi);
+            if (active && !cut) {
+                if (g.pool.whole) tma_load_5d(tile + at, boxes, bar, 0, 0, 0, slot / 8, now);
+                else tma_load_5d(tile + at, boxes, bar, half * 64, slot, 0, 0, now);
+            }
+            if (PLANE == 1) {
                 uint32_t cuts = __ballot_sync(~0u, cut);
                 while (cuts) {
                     const int l = __ffs(cuts) - 1;
                     cuts &= cuts - 1;
-                    const int ck = __shfl_sync(~0u, now_key, l), cp = __shfl_sync(~0u, now, l), cs = __shfl_sync(~0u, slot, l);
-                    const int ch = l / nbox, cb = l - ch * nbox;
-                    char *to = smem + L::kKv + stage * L::kTile + ch * kHalfBytes + cb * g.box * 128;
-                    for (int r = lane; r < g.box; r += 32)
-                        tma_load_5d(to + r * 128, lines, bar, ch * 64, cs + r, run.h, 1, ck + r >= lo && ck + r < hi ? cp : none);
+                    const int ck = __shfl_sync(~0u, now_key, l), ci = __shfl_sync(~0u, now, l), cs = __shfl_sync(~0u, slot, l);
+                    const uint32_t to = __shfl_sync(~0u, at, l);
+                    const int from = g.pool.whole ? 0 : l / nbox, rows = g.box * (g.pool.whole ? kHalves : 1);
+                    for (int e = lane; e < rows; e += 32) {
+                        const int h = e / g.box, row = e - h * g.box;
+                        tma_load_5d(tile + to + h * g.pool.half_bytes + row / 8 * g.pool.group_bytes + row % 8 * 128, lines, bar,
+                                    (from + h) * 64, cs + row, 0, 0, ck + row >= r.lo && ck + row < r.hi ? ci : none);
+                    }
                 }
             }
-            ++n_block;
         }
+        return true;
     }
 
     // ---- warp 9: matrix instructions ----
@@ -323,44 +426,46 @@ struct Kernel {
         const uint32_t qk = mma_desc(kBf16Type, false, kBlockKeys);
         const uint32_t pv = mma_desc(kBf16Type, true, ksteps * 16);
         const uint32_t base = smem_u32(smem);
+        const uint32_t group = g.pool.group_bytes, halves = g.pool.half_bytes;
         int n_run = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
         int64_t kv0 = 0;
         for (;;) {
             const RunInfo r = take_run(n_run);
             if (!r.blocks) break;
-            const int n[2] = {r.pair ? r.blocks : (r.blocks + 1) / 2, r.pair ? r.blocks : r.blocks / 2};
-            for (int t = 0; t <= r.pair; ++t) wait(&c->q_full[t], n_q[t]++ & 1);
+            const bool pair = r.tokens > g.shape.tokens_stream;
+            const int n[2] = {pair ? r.blocks : (r.blocks + 1) / 2, pair ? r.blocks : r.blocks / 2};
+            for (int t = 0; t <= pair; ++t) wait(&c->q_full[t], n_q[t]++ & 1);
             auto scores = [&](int s, int i) {
-                const int block = r.pair ? i : 2 * i + s;
+                const int block = pair ? i : 2 * i + s;
                 const int64_t idx = kv0 + 2 * block;
                 const int stage = static_cast<int>(idx % L::kStages);
                 wait(&c->kv_full[stage], (idx / L::kStages) & 1);
                 tmem_fence_after();
-                if (lane == 0) {
-                    const uint32_t qa = base + L::kQ + (r.pair ? s : 0) * L::kTile, ka = base + L::kKv + stage * L::kTile;
-                    for (int e = 0; e < ksteps; ++e) {
-                        const uint32_t off = (e >> 2) * kHalfBytes + (e & 3) * 32;
-                        mma_ss(tmem + s_at(s), smem_tile_desc(qa + off, 16, 1024), smem_tile_desc(ka + off, 16, 1024), qk, e > 0);
-                    }
-                    if (!r.pair || s == 1) mma_commit(&c->kv_empty[stage]);
-                    if (r.pair ? i + 1 == n[s] : block + 1 == r.blocks) mma_commit(&c->q_empty[r.pair ? s : 0]);
+                if (elect_one()) {
+                    const uint64_t qd = smem_tile_desc(base + L::kQ + (pair ? s : 0) * L::kTile, 16, 1024);
+                    const uint64_t kd = smem_tile_desc(base + L::kKv + stage * L::kTile, 16, group);
+                    for (int e = 0; e < ksteps; ++e)
+                        mma_ss(tmem + s_at(s), qd + ((e >> 2) * kHalfBytes + (e & 3) * 32) / 16,
+                               kd + ((e >> 2) * halves + (e & 3) * 32) / 16, qk, e > 0);
+                    if (!pair || s == 1) mma_commit(&c->kv_empty[stage]);
+                    if (pair ? i + 1 == n[s] : block + 1 == r.blocks) mma_commit(&c->q_empty[pair ? s : 0]);
                     mma_commit(&c->s_full[s]);
                 }
                 __syncwarp();
             };
             auto values = [&](int s, int i) {
-                const int block = r.pair ? i : 2 * i + s;
+                const int block = pair ? i : 2 * i + s;
                 const int64_t idx = kv0 + 2 * block + 1;
                 const int stage = static_cast<int>(idx % L::kStages);
                 wait(&c->kv_full[stage], (idx / L::kStages) & 1);
                 wait(&c->p_full[s], n_p[s]++ & 1);
                 tmem_fence_after();
-                if (lane == 0) {
-                    const uint32_t va = base + L::kKv + stage * L::kTile;
+                if (elect_one()) {
+                    const uint64_t vd = smem_tile_desc(base + L::kKv + stage * L::kTile, halves, group);
+#pragma unroll
                     for (int e = 0; e < kBlockKeys / 16; ++e)
-                        mma_ts(tmem + o_at(s), tmem + s_at(s) + e * 8, smem_tile_desc(va + e * 2048, kHalfBytes, 1024), pv,
-                               i > 0 || e > 0);
-                    if (!r.pair || s == 1) mma_commit(&c->kv_empty[stage]);
+                        mma_ts(tmem + o_at(s), tmem + s_at(s) + e * 8, vd + e * (group / 8), pv, i > 0 || e > 0);
+                    if (!pair || s == 1) mma_commit(&c->kv_empty[stage]);
                     if (i + 1 == n[s]) mma_commit(&c->o_full[s]);
                 }
                 __syncwarp();
@@ -378,7 +483,7 @@ struct Kernel {
         }
         if (gave_up()) {
             // instructions may be in flight whose end nobody has seen: tensor memory stays ours until then
-            if (lane == 0) {
+            if (elect_one()) {
                 mma_commit(&c->drain);
                 mbar_wait_bounded(&c->drain, 0, g.budget);
             }
@@ -386,43 +491,35 @@ struct Kernel {
         }
     }
 
-    // ---- warps 10, 11: queries ----
-    __device__ void query_loop(int t) const {
-        constexpr int kChunks = DP / 8;
+    // ---- warp 10: queries ----
+    __device__ void query_loop(const CUtensorMap *queries) const {
         const PagedAttentionArgs &a = g.a;
-        const T *q = static_cast<const T *>(a.q);
+        const int each = g.shape.parts / a.kv_heads, tokens = g.shape.tokens_stream;
         int n_run = 0, n_q[2] = {0, 0};
         for (;;) {
             const RunInfo r = take_run(n_run);
             if (!r.blocks) break;
-            for (int half = 0; half <= r.pair; ++half) {
-                wait(&c->q_empty[half], (n_q[half]++ & 1) ^ 1);
-                const int left = r.rows - half * kStreamRows;
-                const int todo = (left < kStreamRows ? left : kStreamRows) * kChunks;
-                char *tile = smem + L::kQ + half * L::kTile;
-#pragma unroll 4
-                for (int e = t; e < todo; e += 64) {
-                    const int row = e / kChunks, chunk = e % kChunks;
-                    const int at = r.r0 + half * kStreamRows + row;
-                    const int token = at / g.shape.group, head = r.h * g.shape.group + at - token * g.shape.group;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (chunk * 8 < a.dim)
-                        v = *reinterpret_cast<const uint4 *>(q + (r.q0 + token) * a.q_st + head * a.q_sh + chunk * 8);
-                    v.x ^= g.negate, v.y ^= g.negate, v.z ^= g.negate, v.w ^= g.negate;
-                    *reinterpret_cast<uint4 *>(tile + (chunk / 8) * kHalfBytes + row * 128 + ((chunk ^ row) & 7) * 16) = v;
+            for (int s = 0; s <= (r.tokens > tokens); ++s) {
+                wait(&c->q_empty[s], (n_q[s]++ & 1) ^ 1);
+                if (!gave_up() && elect_one()) {
+                    mbar_arrive_expect_tx(&c->q_full[s], tokens * g.shape.heads * 128 * kHalves);
+                    for (int h = 0; h < kHalves; ++h)
+                        tma_load_4d(smem + L::kQ + s * L::kTile + h * kHalfBytes, queries, &c->q_full[s], h * 64,
+                                    r.part % each * g.shape.heads, r.part / each, r.q0 + r.t0 + s * tokens);
                 }
-                fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&c->q_full[half]);
             }
         }
+        if (gave_up() && lane == 0)  // as drain_loads
+            for (int s = 0; s < 2; ++s)
+                if (n_q[s]) mbar_wait_bounded(&c->q_full[s], (n_q[s] - 1) & 1, g.budget / 8);
         if (a.fill_tail) {
             // rows of no sequence
             const int n = a.batch.seqs;
             const int head = n ? plan_clamp(a.batch.starts.at(0), 0, a.rows) : static_cast<int>(a.rows);
             const int tail = n ? plan_clamp(a.batch.starts.at(n), head, a.rows) : static_cast<int>(a.rows);
             const int64_t rows = head + a.rows - tail, per = a.q_heads * static_cast<int64_t>(a.dim);
-            for (int64_t i = blockIdx.x * 64 + t; i < rows * per; i += gridDim.x * 64) {
+            for (int64_t i = blockIdx.x * 32 + lane; i < rows * per; i += gridDim.x * 32) {
                 const int64_t k = i / per, e = i - k * per, row = k < head ? k : tail + (k - head);
                 static_cast<T *>(a.out)[row * a.o_st + e / a.dim * a.o_sh + e % a.dim] = from_f32<T>(0.f);
                 if (a.lse && e % a.dim == 0) a.lse[row * a.q_heads + e / a.dim] = -INFINITY;
@@ -438,9 +535,41 @@ struct Kernel {
         return r;
     }
 
+    // Replaces the scores of columns outside [lo, hi) and on boxes that are not there.
+    __device__ __forceinline__ void mask_scores(uint32_t (&x)[4][32], int lo, int hi, uint32_t boxes) const {
+        const int shift = __ffs(g.box) - 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int up = hi - j * 32, down = lo - j * 32;
+            uint32_t seen = up >= 32 ? ~0u : up <= 0 ? 0u : (1u << up) - 1;
+            if (down > 0) seen = down >= 32 ? 0u : seen & (~0u << down);
+            if (boxes != ~0u)
+                for (int e = 0; e < 32; ++e) seen &= ~((~boxes >> ((j * 32 + e) >> shift) & 1u) << e);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                if (!(seen >> e & 1u)) x[j][e] = 0xff800000u;
+        }
+    }
+
+    // The largest of a row's 128 scores, by four chains.
+    static __device__ __forceinline__ float largest(const uint32_t (&x)[4][32]) {
+        float t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            t[j] = fmaxf(__uint_as_float(x[j][0]), __uint_as_float(x[j][1]));
+#pragma unroll
+            for (int e = 2; e < 32; e += 2)
+                t[j] = fmaxf(fmaxf(t[j], __uint_as_float(x[j][e])), __uint_as_float(x[j][e + 1]));
+        }
+        return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+    }
+
     __device__ void softmax_loop(uint32_t tmem, int s) const {
         const PagedAttentionArgs &a = g.a;
+        const PlanShape &shape = g.shape;
         const int warp = (threadIdx.x >> 5) & 3, row = warp * 32 + lane;
+        const int row_token = row / shape.heads, row_head = row - row_token * shape.heads;
+        const int each = shape.parts / a.kv_heads;
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
         const uint32_t ts = tmem + s_at(s) + lanes, to = tmem + o_at(s) + lanes;
         const float scale = g.scale_log2;
@@ -448,20 +577,24 @@ struct Kernel {
         for (;;) {
             const RunInfo r = take_run(n_run);
             if (!r.blocks) break;
-            const int steps = r.pair ? r.blocks : (r.blocks + 1 - s) / 2;
-            const int mine = r.pair ? s * kStreamRows + row : row;  // row of the tile
-            const bool live = mine < r.rows;
+            const bool pair = r.tokens > shape.tokens_stream;
+            const int steps = pair ? r.blocks : (r.blocks + 1 - s) / 2;
+            const int token = pair ? s * shape.tokens_stream + row_token : row_token;  // of the tile
+            const int head_group = r.part % each * shape.heads + row_head;
+            const bool live = row_token < shape.tokens_stream && token < r.tokens && head_group < g.group;
             const bool work = __any_sync(~0u, live);
-            const int token = (r.r0 + mine) / g.shape.group;
             int lo = 0, hi = 1 << 30;  // keys that the row sees
             if (live) {
-                const int at = r.first + token;
+                const int at = r.first + r.t0 + token;
                 hi = a.causal && at + 1 < r.end ? at + 1 : r.end;
-                if (a.window > 0) lo = at + 1 - g.shape.window;
+                if (a.window > 0) lo = at + 1 - shape.window;
             }
+            // keys that every row of the warp sees: blocks inside need no mask
+            const int all_lo = __reduce_max_sync(~0u, lo), all_hi = __reduce_min_sync(~0u, hi);
+            bool huge = false;  // some row's m is too large for one rounding (below)
             float m = -INFINITY, ref = 0.f, sum = 0.f;  // m = ref * scale
             for (int i = 0; i < steps; ++i) {
-                const int block = r.pair ? i : 2 * i + s;
+                const int block = pair ? i : 2 * i + s;
                 const int key0 = r.key0 + block * kBlockKeys;
                 wait(&c->s_full[s], n_s++ & 1);
                 tmem_fence_after();
@@ -469,26 +602,27 @@ struct Kernel {
                     uint32_t x[4][32];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) tmem_ld32(ts + j * 32, x[j]);
-                    tmem_wait_ld();
                     const uint32_t boxes = c->mask[(n_block + block) % kMaskSlots];
-                    if (__any_sync(~0u, live && (hi < key0 + kBlockKeys || lo > key0)) || boxes != ~0u) {
-                        const int up = hi - key0, down = lo - key0, shift = __ffs(g.box) - 1;
+                    tmem_wait_ld();
+                    if (g.negate) {
 #pragma unroll
-                        for (int j = 0; j < 128; ++j)
-                            if (j >= up || j < down || !(boxes >> (j >> shift) & 1)) x[j / 32][j % 32] = 0xff800000u;
+                        for (int j = 0; j < 128; ++j) x[j / 32][j % 32] ^= 0x80000000u;
                     }
-                    float top = __uint_as_float(x[0][0]);
-#pragma unroll
-                    for (int j = 1; j < 128; ++j) top = fmaxf(top, __uint_as_float(x[j / 32][j % 32]));
+                    if (all_hi < key0 + kBlockKeys || all_lo > key0 || boxes != ~0u) mask_scores(x, lo - key0, hi - key0, boxes);
+                    const float top = largest(x);
                     // m, a reference in units of log2
                     const float next = top * scale;
-                    const bool move = next > m + kRescale || (m == -INFINITY && next > m);
+                    const bool move = next > m + kRescale;
                     const float was = m;
-                    if (move) m = next, ref = top;
+                    const bool moves = __any_sync(~0u, move && live);
+                    if (moves) {
+                        if (move) m = next, ref = top;
+                        huge = __any_sync(~0u, live && fabsf(m) > 0x1p24f && m != -INFINITY);
+                    }
                     float less = m == -INFINITY ? 0.f : -m, times = scale;
                     // x * scale - m is off by what m was rounded by, the same for the whole row, so it cancels;
                     // where it could pass 1 (the lowest value of a type as a score) the reference comes off first.
-                    if (__any_sync(~0u, live && fabsf(m) > 0x1p24f && m != -INFINITY)) {
+                    if (huge) {
                         const float off = m == -INFINITY ? 0.f : ref;
 #pragma unroll
                         for (int j = 0; j < 128; ++j)
@@ -496,20 +630,23 @@ struct Kernel {
                         less = 0.f;
                         times = 1.f;
                     }
-                    float add = 0.f;
+                    const Pair times2 = make_pair(times, times), less2 = make_pair(less, less);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint32_t p[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float u = exp2_approx(fmaf(__uint_as_float(x[j][2 * e]), times, less));
-                            const float v = exp2_approx(fmaf(__uint_as_float(x[j][2 * e + 1]), times, less));
-                            add += u + v;
+                            float u, v;
+                            split(fma2(make_pair(x[j][2 * e], x[j][2 * e + 1]), times2, less2), u, v);
+                            u = exp2_approx(u);
+                            v = exp2_approx(v);
                             p[e] = pack(u, v);
+                            x[j][2 * e] = __float_as_uint(u);
+                            x[j][2 * e + 1] = __float_as_uint(v);
                         }
                         tmem_st16(ts + j * 16, p);
                     }
-                    if (i > 0 && __any_sync(~0u, move && live)) {
+                    if (i > 0 && moves) {
                         const float keep = move ? exp2_approx(was - m) : 1.f;
                         sum *= keep;
                         for (int j = 0; j < a.dim; j += 16) {
@@ -521,19 +658,33 @@ struct Kernel {
                             tmem_st16(to + j, o);
                         }
                     }
-                    sum += add;
                     tmem_wait_st();
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&c->p_full[s]);
+                    // the sum is taken while the tensor core has the weights
+                    Pair add[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        add[j] = make_pair(x[j][0], x[j][1]);
+#pragma unroll
+                        for (int e = 2; e < 32; e += 2) add[j] = add2(add[j], make_pair(x[j][e], x[j][e + 1]));
+                    }
+                    float s0, s1;
+                    split(add2(add2(add[0], add[1]), add2(add[2], add[3])), s0, s1);
+                    sum += s0 + s1;
+                } else {
+                    tmem_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&c->p_full[s]);
                 }
-                tmem_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&c->p_full[s]);
             }
             n_block += r.blocks;
             if (steps) {
                 wait(&c->o_full[s], n_o++ & 1);
                 tmem_fence_after();
             }
-            if (!r.pair) {
+            if (!pair) {
                 if (s == 1) {
                     c->join[row][0] = m;
                     c->join[row][1] = sum;
@@ -544,22 +695,23 @@ struct Kernel {
                     wait(&c->join_full, n_join & 1);
                 }
             }
-            if (work && (r.pair || s == 0)) {
+            if (work && (pair || s == 0)) {
                 tmem_fence_after();
                 float k0 = 1.f, k1 = 0.f;
-                const bool both = !r.pair && r.blocks > 1;
+                const bool both = !pair && r.blocks > 1;
                 if (both) {
-                    const float m1 = c->join[row][0], all = fmaxf(m, m1), ref = all == -INFINITY ? 0.f : all;
-                    k0 = exp2_approx(m - ref);
-                    k1 = exp2_approx(m1 - ref);
+                    const float m1 = c->join[row][0], all = fmaxf(m, m1), base = all == -INFINITY ? 0.f : all;
+                    k0 = exp2_approx(m - base);
+                    k1 = exp2_approx(m1 - base);
                     sum = sum * k0 + c->join[row][1] * k1;
                     m = all;
                 }
-                const int64_t q_row = r.q0 + token;
-                const int head = r.h * g.shape.group + (r.r0 + mine - token * g.shape.group);
-                char *slot = static_cast<char *>(a.workspace) + parts_bytes(g.ctas) + (2 * blockIdx.x + r.part) * slot_bytes(DP);
+                const int64_t q_row = r.q0 + r.t0 + token;
+                const int head = r.part / each * g.group + head_group;
+                const int slot_row = (pair ? s * kStreamRows : 0) + row;
+                char *slot = static_cast<char *>(a.workspace) + shared_bytes(g.ctas) + (2 * blockIdx.x + r.slot) * slot_bytes(DP);
                 T *out = static_cast<T *>(a.out) + q_row * a.o_st + head * a.o_sh;
-                if (r.part < 0) {
+                if (r.slot < 0) {
                     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
                     k0 *= inv;
                     k1 *= inv;
@@ -582,7 +734,7 @@ struct Kernel {
                         for (int e = 0; e < 16; ++e) f[e] = 0.f;
                     }
                     if (!live) continue;
-                    if (r.part < 0) {
+                    if (r.slot < 0) {
 #pragma unroll
                         for (int e = 0; e < 16; e += 8)
                             if (j + e < a.dim)
@@ -590,18 +742,18 @@ struct Kernel {
                                     make_uint4(pack(f[e], f[e + 1]), pack(f[e + 2], f[e + 3]), pack(f[e + 4], f[e + 5]),
                                                pack(f[e + 6], f[e + 7]));
                     } else {
-                        float *o32 = reinterpret_cast<float *>(slot) + mine * DP + j;
+                        float *o32 = reinterpret_cast<float *>(slot) + slot_row * DP + j;
 #pragma unroll
                         for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4 *>(o32 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
                     }
                 }
-                if (live && r.part >= 0)
-                    reinterpret_cast<float2 *>(slot + static_cast<size_t>(kTileRows) * DP * 4)[mine] = make_float2(m, sum);
-                if (live && r.part < 0 && a.lse)
+                if (live && r.slot >= 0)
+                    reinterpret_cast<float2 *>(slot + static_cast<size_t>(2 * kStreamRows) * DP * 4)[slot_row] = make_float2(m, sum);
+                if (live && r.slot < 0 && a.lse)
                     a.lse[q_row * a.q_heads + head] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
                 tmem_fence_before();
             }
-            if (!r.pair) {
+            if (!pair) {
                 // stream 1's output has been read before its next weights can overwrite it
                 if (s == 0) {
                     __syncwarp();
@@ -618,7 +770,7 @@ struct Kernel {
 template <int DP, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_attention_kernel(const __grid_constant__ KernelArgs g, const __grid_constant__ CUtensorMap boxes,
-                           const __grid_constant__ CUtensorMap lines) {
+                           const __grid_constant__ CUtensorMap lines, const __grid_constant__ CUtensorMap queries) {
     using K = Kernel<DP, T>;
     extern __shared__ __align__(1024) char raw[];
     typename K::C *c = reinterpret_cast<typename K::C *>(raw + K::L::kControl);
@@ -633,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&c->kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&c->q_full[i], 2);
+            mbar_init(&c->q_full[i], 1);
             mbar_init(&c->q_empty[i], 1);
             mbar_init(&c->s_full[i], 1);
             mbar_init(&c->p_full[i], 4);
@@ -652,6 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_prefetch_map(&boxes);
             tma_prefetch_map(&lines);
         }
+        tma_prefetch_map(&queries);
     }
     tmem_fence_before();
     __syncthreads();
@@ -659,9 +812,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = c->tmem;
     pdl_launch();
     if (warp < 8) k.softmax_loop(tmem, warp >> 2);
-    else if (warp == 8) k.load_loop(&boxes, &lines);
+    else if (warp == 8) k.plan_loop(&boxes, &lines);
     else if (warp == 9) k.mma_loop(tmem);
-    else k.query_loop(threadIdx.x - 320);
+    else if (warp == 10) k.query_loop(&queries);
+    else k.value_loop(&boxes, &lines);
     tmem_fence_before();
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
@@ -671,23 +825,30 @@ __global__ void __launch_bounds__(kThreads, 1)
 // CTA c and does not end there, the y-th part of its rows.
 constexpr int kJoinThreads = 128;
 template <int DP, typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const __grid_constant__ KernelArgs g) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ KernelArgs g) {
     pdl_wait();
     const PagedAttentionArgs &a = g.a;
-    const Part p = static_cast<const Part *>(a.workspace)[blockIdx.x];
-    if (p.pieces < 2) return;
+    const Shared p = static_cast<const Shared *>(a.workspace)[blockIdx.x];
+    const int pieces = min(p.pieces, static_cast<int>(gridDim.x - blockIdx.x));
+    if (pieces < 2) return;
     constexpr int kLanes = DP / 4;
-    const int e = threadIdx.x % kLanes * 4;
-    const char *slots = static_cast<const char *>(a.workspace) + parts_bytes(g.ctas);
-    for (int r = blockIdx.y * (kJoinThreads / kLanes) + threadIdx.x / kLanes; r < p.rows; r += gridDim.y * (kJoinThreads / kLanes)) {
+    const int e = threadIdx.x % kLanes * 4, each = g.shape.parts / a.kv_heads, step = gridDim.y * (kJoinThreads / kLanes);
+    const char *slots = static_cast<const char *>(a.workspace) + shared_bytes(g.ctas);
+    for (int n = blockIdx.y * (kJoinThreads / kLanes) + threadIdx.x / kLanes; n < p.tokens * g.shape.heads; n += step) {
+        const int token = n / g.shape.heads, row_head = n - token * g.shape.heads;
+        const int stream = token >= g.shape.tokens_stream;
+        const int r = stream * kStreamRows + (token - stream * g.shape.tokens_stream) * g.shape.heads + row_head;
+        const int head_group = p.part % each * g.shape.heads + row_head;
+        if (head_group >= g.group) continue;
         float m = -INFINITY, sum = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < p.pieces; ++i) {
+#pragma unroll 4
+        for (int i = 0; i < pieces; ++i) {
             const char *slot = slots + (2 * static_cast<size_t>(blockIdx.x + i) + (i == 0)) * slot_bytes(DP);
-            const float2 ms = reinterpret_cast<const float2 *>(slot + static_cast<size_t>(kTileRows) * DP * 4)[r];
+            const float2 ms = reinterpret_cast<const float2 *>(slot + static_cast<size_t>(2 * kStreamRows) * DP * 4)[r];
             const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(slot) + r * DP + e);
-            const float all = fmaxf(m, ms.x), ref = all == -INFINITY ? 0.f : all;
-            const float k0 = exp2_approx(m - ref), k1 = exp2_approx(ms.x - ref);
+            const float all = fmaxf(m, ms.x), base = all == -INFINITY ? 0.f : all;
+            const float k0 = exp2_approx(m - base), k1 = exp2_approx(ms.x - base);
             m = all;
             sum = sum * k0 + ms.y * k1;
             o.x = o.x * k0 + v.x * k1;
@@ -696,24 +857,20 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const __grid_c
             o.w = o.w * k0 + v.w * k1;
         }
         const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-        const int token = (p.r0 + r) / g.shape.group, head = p.h * g.shape.group + p.r0 + r - token * g.shape.group;
-        const int64_t row = p.q0 + token;
-        if (e < a.dim) {
-            T *out = static_cast<T *>(a.out) + row * a.o_st + head * a.o_sh + e;
-            const uint2 v = make_uint2(Kernel<DP, T>::pack(o.x * inv, o.y * inv), Kernel<DP, T>::pack(o.z * inv, o.w * inv));
-            *reinterpret_cast<uint2 *>(out) = v;
-        }
+        const int64_t row = p.q0 + p.t0 + token;
+        const int head = p.part / each * g.group + head_group;
+        if (e < a.dim)
+            *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + row * a.o_st + head * a.o_sh + e) =
+                make_uint2(Kernel<DP, T>::pack(o.x * inv, o.y * inv), Kernel<DP, T>::pack(o.z * inv, o.w * inv));
         if (a.lse && e == 0) a.lse[row * a.q_heads + head] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
     }
 }
 
 // CTAs that a call is given: no more than its units can be, and one an SM.
-int plan_ctas(const PagedAttentionArgs &a, int sms) {
-    const int64_t group = a.q_heads / a.kv_heads;
-    const int64_t tokens = a.batch.table_width * a.batch.page_tokens;
-    const int64_t blocks = tokens > kBlockKeys ? (tokens + kBlockKeys - 1) / kBlockKeys : 1;
+int plan_ctas(const PagedAttentionArgs &a, const PlanShape &s, int sms) {
+    const int64_t blocks = s.tokens > kBlockKeys ? (s.tokens + kBlockKeys - 1) / kBlockKeys : 1;
     const int64_t seqs = a.batch.seqs < a.rows ? a.batch.seqs : a.rows;
-    const int64_t tiles = (seqs + a.rows * group / kTileRows) * a.kv_heads;
+    const int64_t tiles = (seqs + a.rows / (2 * s.tokens_stream)) * s.parts;
     const int64_t units = blocks > sms || tiles > sms ? sms : tiles * blocks;
     return static_cast<int>(units < 1 ? 1 : units < sms ? units : sms);
 }
@@ -722,34 +879,71 @@ using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, vo
                               const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// The pool as (element, slot, key head, plane, page), in boxes of `tokens` slots of 64 elements.
-int encode_pool(const PagedAttentionArgs &a, int dtype, int tokens, CUtensorMap *map) {
-    static const auto encode = reinterpret_cast<EncodeFn>(gpu::driver_symbol("cuTensorMapEncodeTiled"));
-    if (!encode) return cudaErrorNotSupported;
-    const cuuint64_t dims[5] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.batch.page_tokens),
-                                static_cast<cuuint64_t>(a.kv_heads), 2, static_cast<cuuint64_t>(a.batch.pages)};
-    const cuuint64_t strides[4] = {static_cast<cuuint64_t>(a.pool_token) * 2, static_cast<cuuint64_t>(a.pool_head) * 2,
-                                   static_cast<cuuint64_t>(a.pool_plane) * 2, static_cast<cuuint64_t>(a.pool_page) * 2};
-    const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(tokens), 1, 1, 1}, one[5] = {1, 1, 1, 1, 1};
-    const CUresult e = encode(map, dtype == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
-                              const_cast<void *>(a.pool), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+int encode(int dtype, void *base, int rank, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box,
+           CUtensorMap *map) {
+    static const auto fn = reinterpret_cast<EncodeFn>(gpu::driver_symbol("cuTensorMapEncodeTiled"));
+    if (!fn) return cudaErrorNotSupported;
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    const CUresult e = fn(map, dtype == kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank, base,
+                          dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return e == CUDA_SUCCESS ? 0 : static_cast<int>(cudaErrorInvalidValue);
 }
 
+// The pool's index and its maps: boxes of g->box slots, and lines of one.
+int view_pool(KernelArgs *g, int dtype, CUtensorMap *boxes, CUtensorMap *lines) {
+    const PagedAttentionArgs &a = g->a;
+    const int64_t page = a.batch.pages > 1 ? a.pool_page : 0, head = a.kv_heads > 1 ? a.pool_head : 0;
+    int64_t unit = a.pool_plane;
+    for (int64_t other : {page, head})
+        while (other) {
+            const int64_t rest = unit % other;
+            unit = other;
+            other = rest;
+        }
+    if (unit <= 0 || unit % 8) return cudaErrorInvalidValue;
+    const int64_t last = ((a.batch.pages - 1) * page + a.pool_plane + (a.kv_heads - 1) * head) / unit;
+    if (last >= 0x7fffffff) return cudaErrorInvalidValue;
+    g->pool.page = static_cast<int>(page / unit);
+    g->pool.plane = static_cast<int>(a.pool_plane / unit);
+    g->pool.head = static_cast<int>(head / unit);
+    g->pool.none = static_cast<int>(last + 1);
+    void *base = const_cast<void *>(a.pool);
+    const cuuint64_t token = static_cast<cuuint64_t>(a.pool_token) * 2, index = static_cast<cuuint64_t>(unit) * 2;
+    const cuuint64_t dim = a.dim, slots = a.batch.page_tokens, all = static_cast<cuuint64_t>(last) + 1;
+    const cuuint32_t box = g->box;
+    const cuuint64_t dims[5] = {dim, slots, 1, 1, all}, strides[4] = {token, token * slots, token * slots, index};
+    const cuuint32_t line[5] = {64, 1, 1, 1, 1}, rows[5] = {64, box, 1, 1, 1};
+    int e = encode(dtype, base, 5, dims, strides, line, lines);
+    if (e) return e;
+    if (!g->pool.whole) return encode(dtype, base, 5, dims, strides, rows, boxes);
+    const cuuint64_t dims_whole[5] = {64, 8, dim / 64, slots / 8, all}, strides_whole[4] = {token, 128, token * 8, index};
+    const cuuint32_t box_whole[5] = {64, 8, static_cast<cuuint32_t>(dim / 64), box / 8, 1};
+    return encode(dtype, base, 5, dims_whole, strides_whole, box_whole, boxes);
+}
+
+// The queries as (element, query head of a key head, key head, token), a stream's rows a box.
+int view_queries(const KernelArgs &g, int dtype, CUtensorMap *queries) {
+    const PagedAttentionArgs &a = g.a;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(g.group),
+                                static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.rows)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(a.q_sh) * 2, static_cast<cuuint64_t>(a.q_sh) * g.group * 2,
+                                   static_cast<cuuint64_t>(a.q_st) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(g.shape.heads), 1, static_cast<cuuint32_t>(g.shape.tokens_stream)};
+    return encode(dtype, const_cast<void *>(a.q), 4, dims, strides, box, queries);
+}
+
 template <int DP, typename T>
-int launch(const KernelArgs &g, int dtype, int device, bool join, cudaStream_t st) {
+int launch(KernelArgs &g, int dtype, int device, bool join, cudaStream_t st) {
     using K = Kernel<DP, T>;
     constexpr int smem = K::L::kControl + static_cast<int>(sizeof(typename K::C));
     static_assert(smem <= 227 * 1024, "shared memory of one CTA");
-    CUtensorMap boxes, lines;
+    CUtensorMap boxes, lines, queries;
     std::memset(&boxes, 0, sizeof boxes);
     std::memset(&lines, 0, sizeof lines);
-    if (g.a.batch.pages) {
-        int e = encode_pool(g.a, dtype, g.box, &boxes);
-        if (!e) e = encode_pool(g.a, dtype, 1, &lines);
-        if (e) return e;
-    }
+    int bad = g.a.batch.pages ? view_pool(&g, dtype, &boxes, &lines) : 0;
+    if (!bad) bad = view_queries(g, dtype, &queries);
+    if (bad) return bad;
     static std::atomic<uint64_t> configured{0};  // devices
     cudaError_t e = cudaSuccess;
     if (device > 63 || !(configured.load(std::memory_order_acquire) >> device & 1)) {
@@ -757,7 +951,7 @@ int launch(const KernelArgs &g, int dtype, int device, bool join, cudaStream_t s
         if (e != cudaSuccess) return static_cast<int>(e);
         if (device <= 63) configured.fetch_or(1ull << device, std::memory_order_release);
     }
-    paged_attention_kernel<DP, T><<<g.ctas, kThreads, smem, st>>>(g, boxes, lines);
+    paged_attention_kernel<DP, T><<<g.ctas, kThreads, smem, st>>>(g, boxes, lines, queries);
     note_launch();
     e = cudaGetLastError();
     if (e != cudaSuccess || !join) return static_cast<int>(e);
@@ -770,7 +964,7 @@ int launch(const KernelArgs &g, int dtype, int device, bool join, cudaStream_t s
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, join_parts_kernel<DP, T>, g);
+    e = cudaLaunchKernelEx(&cfg, join_kernel<DP, T>, g);
     note_launch();
     return static_cast<int>(e);
 }
@@ -780,7 +974,7 @@ int launch(const KernelArgs &g, int dtype, int device, bool join, cudaStream_t s
 size_t paged_attention_workspace(int64_t rows, int q_heads, int kv_heads, int dim, int seqs, int device) {
     (void)rows, (void)q_heads, (void)kv_heads, (void)seqs;
     const int sms = sm_count(device);
-    return parts_bytes(sms) + 2 * static_cast<size_t>(sms) * slot_bytes(dim <= 64 ? 64 : 128);
+    return shared_bytes(sms) + 2 * static_cast<size_t>(sms) * slot_bytes(dim <= 64 ? 64 : 128);
 }
 
 int paged_attention(const PagedAttentionArgs &a, int dtype, int device, void *stream) {
@@ -793,20 +987,26 @@ int paged_attention(const PagedAttentionArgs &a, int dtype, int device, void *st
     KernelArgs g;
     g.a = a;
     const int64_t tokens = a.batch.pages > 0 ? a.batch.table_width * a.batch.page_tokens : 0;
-    g.shape.group = a.q_heads / a.kv_heads;
-    g.shape.kv_heads = a.kv_heads;
+    g.group = a.q_heads / a.kv_heads;
+    plan_parts(&g.shape, a.kv_heads, g.group);
     g.shape.causal = a.causal;
     g.shape.window = plan_clamp(a.window, 0, kMostTokens);
     g.shape.rows = static_cast<int>(a.rows);
     g.shape.tokens = plan_clamp(tokens, 0, kMostTokens);
     // a scale of zero would make NaN of a masked score; this one gives every seen score the same weight
     g.scale_log2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
-    g.negate = a.scale < 0.f ? 0x80008000u : 0u;
+    g.negate = a.scale < 0.f;
     g.box = a.batch.page_tokens & -a.batch.page_tokens;
     if (g.box > kBlockKeys) g.box = kBlockKeys;
+    g.page_tokens = FastDiv(static_cast<uint32_t>(a.batch.page_tokens));
+    g.pool = PoolView();
+    g.pool.whole = a.dim % 64 == 0;
+    const int halves = a.dim <= 64 ? 1 : 2, tile_half = kStreamRows * 128;
+    g.pool.group_bytes = g.pool.whole ? 1024 * halves : 1024;
+    g.pool.half_bytes = g.pool.whole ? 1024 : tile_half;
     g.budget = wait_budget_ns();
-    g.ctas = plan_ctas(a, sm_count(device));
-    if (!a.workspace || a.workspace_bytes < parts_bytes(g.ctas) + 2 * g.ctas * slot_bytes(a.dim <= 64 ? 64 : 128))
+    g.ctas = plan_ctas(a, g.shape, sm_count(device));
+    if (!a.workspace || a.workspace_bytes < shared_bytes(g.ctas) + 2 * g.ctas * slot_bytes(a.dim <= 64 ? 64 : 128))
         return cudaErrorInvalidValue;
     const bool join = g.ctas > 1 && tokens > kBlockKeys;  // a tile of one block is never shared
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -217,6 +217,11 @@ def _batch(pool, page_table, seq_lens, query_starts, device):
             query_starts.data_ptr(), kinds[2], seqs, pool.shape[3], pool.shape[0])
 
 
+def _strides(t: torch.Tensor):
+    """Strides, with those of axes of one element (which are not used) aligned."""
+    return tuple(st if n > 1 else 8 for n, st in zip(t.shape[:-1], t.stride())) + (t.stride(-1),)
+
+
 def _rows(t: torch.Tensor, what: str, pool: torch.Tensor, device: torch.device) -> None:
     if t.dim() != 3 or t.dtype != pool.dtype or t.device != device or t.shape[2] != pool.shape[4]:
         raise ValueError(f"{what} must be a [tokens, heads, {pool.shape[4]}] {pool.dtype} tensor on {device}")
@@ -327,10 +332,10 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
         raise ValueError("head_dim must be a multiple of 8 up to 128, page_tokens a multiple of 8")
     if window < 0 or (window and not causal):
         raise ValueError("window must be positive, and needs causal")
-    ps, qs = pool.stride(), q.stride()
+    ps, qs = _strides(pool), _strides(q)
     if ps[4] != 1 or (ps[0] | ps[1] | ps[2] | ps[3]) % 8 or pool.data_ptr() % 16 or min(ps) < 1:
         raise ValueError("the cache must have unit stride in a head and 16-byte aligned strides otherwise")
-    if qs[2] != 1 or (qs[0] | qs[1]) % 8 or q.data_ptr() % 16:
+    if qs[2] != 1 or (qs[0] | qs[1]) % 8 or q.data_ptr() % 16 or min(qs) < 1:
         raise ValueError("q must have unit stride in a head and 16-byte aligned strides otherwise")
     fresh = out is None
     if fresh:
@@ -341,7 +346,7 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
         if out.shape != q.shape:
             raise ValueError("out must have the shape of q")
         _own_memory(out, "out")
-    os = out.stride()
+    os = _strides(out)
     if os[2] != 1 or (os[0] | os[1]) % 8 or out.data_ptr() % 16:
         raise ValueError("out must have unit stride in a head and 16-byte aligned strides otherwise")
     _on_gpu("paged_attention", device)

@@ -54,6 +54,13 @@ static void test_places() {
     }
 }
 
+static void test_div() {
+    const int64_t v[] = {0, 1, 2, 7, 255, 0x7fffffff, 0xffffffffll, 0x100000000ll, 0x123456789abll, INT64_MAX};
+    for (int64_t a : v)
+        for (int64_t b : v)
+            if (b) CHECK(plan_div(a, b) == a / b);
+}
+
 static void check_plan(const PlanShape &s, const std::vector<int64_t> &starts, const std::vector<int64_t> &lens, int ctas) {
     const int seqs = static_cast<int>(lens.size());
     std::vector<PlanSeq> q;
@@ -62,15 +69,17 @@ static void check_plan(const PlanShape &s, const std::vector<int64_t> &starts, c
         q.push_back(plan_seq(s, starts[b], starts[b + 1], lens[b]));
         CHECK(q[b].q0 >= 0 && q[b].new_tokens >= 0 && q[b].q0 + q[b].new_tokens <= s.rows);
         CHECK(q[b].end >= 0 && q[b].end <= s.tokens);
-        units += s.kv_heads * plan_head_units(s, q[b]);
+        units += s.parts * plan_part_units(s, q[b]);
+        int tokens = 0;
         for (int m = 0; m < q[b].tiles; ++m) {
             const PlanTile t = plan_tile(s, q[b], m);
-            CHECK(t.rows > 0 && t.rows <= kTileRows && t.blocks > 0 && t.block0 >= 0);
+            CHECK(t.tokens > 0 && t.tokens <= 2 * s.tokens_stream && t.blocks > 0 && t.block0 >= 0);
             CHECK(t.lo >= 0 && t.hi <= q[b].end && t.lo <= t.hi);
             CHECK(t.block0 * kBlockKeys <= t.lo && (t.block0 + t.blocks) * kBlockKeys >= t.hi);
+            tokens += t.tokens;
             int lo = 1 << 30, hi = 0;
-            for (int r = 0; r < t.rows; ++r) {
-                const int at = q[b].first + (m * kTileRows + r) / s.group;
+            for (int r = 0; r < t.tokens; ++r) {
+                const int at = q[b].first + m * 2 * s.tokens_stream + r;
                 int to = q[b].end, from = 0;
                 if (s.causal && at + 1 < to) to = at + 1;
                 if (s.window && at + 1 - s.window > 0) from = at + 1 - s.window;
@@ -81,6 +90,8 @@ static void check_plan(const PlanShape &s, const std::vector<int64_t> &starts, c
             }
             if (hi) CHECK(t.lo <= lo && t.hi >= hi);
         }
+        CHECK(tokens == q[b].new_tokens);
+        CHECK(plan_part_units(s, q[b]) == plan_part_units(s, q[b], 0, 3) + plan_part_units(s, q[b], 1, 3) + plan_part_units(s, q[b], 2, 3));
     }
     const int64_t share = plan_share(units, ctas);
     CHECK(share * ctas >= units);
@@ -91,12 +102,15 @@ static void check_plan(const PlanShape &s, const std::vector<int64_t> &starts, c
         int b = 0;
         int64_t head = 0;
         for (;; ++b) {
-            head = plan_head_units(s, q[b]);
-            if (begin < s.kv_heads * head) break;
-            begin -= s.kv_heads * head;
+            head = plan_part_units(s, q[b]);
+            if (begin < s.parts * head) break;
+            begin -= s.parts * head;
         }
         PlanCursor cur;
-        cur.seek(s, q[b], head, begin);
+        cur.part = static_cast<int>(plan_div(begin, head));
+        begin -= cur.part * head;
+        for (; begin >= plan_tile(s, q[b], cur.m).blocks; ++cur.m) begin -= plan_tile(s, q[b], cur.m).blocks;
+        cur.block = static_cast<int>(begin);
         while (left > 0) {
             PlanRun run;
             if (!cur.next(s, q[b], left, &run)) {
@@ -106,7 +120,7 @@ static void check_plan(const PlanShape &s, const std::vector<int64_t> &starts, c
                 continue;
             }
             CHECK(run.from < run.to && run.to <= run.tile.blocks);
-            for (int i = run.from; i < run.to; ++i) ++done[{b, run.h, run.m, i}];
+            for (int i = run.from; i < run.to; ++i) ++done[{b, run.part, run.m, i}];
             left -= run.to - run.from;
         }
     }
@@ -119,8 +133,11 @@ static void test_plan() {
     auto pick = [&](int lo, int hi) { return lo + static_cast<int>(rng() % (hi - lo + 1)); };
     for (int t = 0; t < 400; ++t) {
         PlanShape s;
-        s.group = pick(1, t % 5 ? 9 : 300);
-        s.kv_heads = pick(1, 4);
+        const int group = pick(1, t % 5 ? 9 : 300), kv_heads = pick(1, 4);
+        plan_parts(&s, kv_heads, group);
+        CHECK(s.parts % kv_heads == 0 && s.heads * s.tokens_stream <= kStreamRows && s.tokens_stream > 0);
+        const int each = s.parts / kv_heads;  // every query head is in one part of its key head
+        CHECK(s.heads * each >= group && s.heads * (each - 1) < group);
         s.causal = t % 4 != 0;
         s.window = s.causal && t % 3 == 0 ? pick(1, 700) : 0;
         s.tokens = pick(0, 2000);
@@ -143,6 +160,7 @@ static void test_plan() {
 
 int main() {
     test_places();
+    test_div();
     test_plan();
     std::printf("ok: %ld checks\n", g_checks);
     return 0;
