@@ -7,20 +7,22 @@
 //
 // One persistent CTA an SM goes through its part of the plan
 // (attention_plan.h) in one pass over the keys. Two streams of 128 rows run
-// against each other so that the tensor core works on one while the other's
-// softmax is computed: stream s has the scores S_s (128 x 128, fp32) and the
-// output O_s (128 x dim, fp32) in tensor memory, and the weights P_s, 16-bit,
-// in place of S_s. A tile of more than 128 rows gives each stream half of its
-// rows, over the same keys. A smaller one (single tokens) gives both streams
+// against each other: stream s has two buffers of scores (128 x 64, fp32) and
+// the output O_s (128 x dim, fp32) in tensor memory, and the weights, 16-bit, in
+// place of their scores. While a stream's softmax works in one buffer the tensor
+// core fills the other and multiplies the other stream's weights. Each stream
+// has its own warp that issues its matrix instructions: the queue of the tensor
+// core is short, and one warp for both would wait in it with one stream's while
+// the other's weights are ready. A tile of more than 128 rows gives each stream
+// half of its rows, over the same keys. A smaller one (single tokens) gives both streams
 // the same rows and every second block of keys, and they are joined at the
 // end, so the loads never wait for one stream's softmax.
 //
 //   warps 0-3, 4-7  the softmax of stream 0, 1: a thread has a row
 //   warp 8          walks the plan, loads K blocks by TMA (a page, or the
 //                   part of one that lies in the block, a box)
-//   warp 9          issues the matrix instructions
-//   warp 10         loads the queries
-//   warp 11         loads V blocks
+//   warps 9, 10     issue the matrix instructions of stream 0, 1
+//   warp 11         loads the queries and V blocks
 //
 // Weights are rounded to the cache's type for the second product; sums,
 // maxima, scores and outputs are 32-bit. m only moves when a score passes it
@@ -44,10 +46,16 @@ namespace kern {
 namespace {
 
 constexpr int kThreads = 384;
+constexpr int kHalfKeys = kBlockKeys / 2;  // keys of a buffer of scores
+// Registers a thread: at launch, then of the softmax's warps, which hold a row
+// of scores, and of the others. What is taken is no more than what is given.
+constexpr int kRegsLaunch = 168, kRegsSoftmax = 200, kRegsOther = 104;
+static_assert(256 * kRegsSoftmax + 128 * kRegsOther <= kThreads * kRegsLaunch, "registers of a CTA");
 constexpr int kRunSlots = 4;
 constexpr int kFewTiles = 4;  // of a sequence, that one lane counts
 constexpr int kMaskSlots = 16;  // blocks whose masks are kept: more than are ever in flight
 constexpr float kRescale = 8.f;
+constexpr int kFmaPairs = 2;  // of 16 pairs of scores, whose exponentials are taken on the FMA pipes
 
 __device__ uint32_t g_attention_status;
 
@@ -79,8 +87,9 @@ template <int STAGES>
 struct Control {
     uint64_t kv_full[STAGES], kv_empty[STAGES];
     uint64_t q_full[2], q_empty[2];
-    uint64_t s_full[2], p_full[2], o_full[2];
-    uint64_t join_full, join_empty, drain;
+    uint64_t s_full[2][2], p_full[2][2], o_step[2], o_full[2];  // o_step: after each half block, o_full: after a run's last
+    uint64_t turn[2][4];  // of a warp's exponentials
+    uint64_t join_full, join_empty, drain[2];
     uint64_t run_full[kRunSlots], run_empty[kRunSlots];
     uint32_t mask[kMaskSlots];  // good boxes of a block
     RunInfo run[kRunSlots];
@@ -130,13 +139,14 @@ struct KernelArgs {
     PagedAttentionArgs a;
     PlanShape shape;
     PoolView pool;
-    FastDiv page_tokens;
+    FastDiv page_tokens, each;  // each: parts of a key head
     int group;         // query heads of a key head
     float scale_log2;  // |scale| * log2(e)
-    int negate;        // scale is negative
     int ctas;
     int box;  // tokens of a full box
-    uint64_t budget;
+    int box_shift;  // a block has 2^box_shift boxes
+    uint64_t budget;  // of a wait, ns
+    uint32_t tries;   // the same, in tries of a microsecond
 };
 
 template <int DP, typename T>
@@ -146,7 +156,7 @@ struct Kernel {
     static constexpr int kHalves = DP / 64;
     static constexpr int kHalfBytes = kStreamRows * 128;
     // columns of tensor memory: scores and weights, output of a stream
-    static __device__ __forceinline__ uint32_t s_at(int s) { return s * 128; }
+    static __device__ __forceinline__ uint32_t s_at(int s, int half) { return s * 128 + half * 64; }
     static __device__ __forceinline__ uint32_t o_at(int s) { return 256 + s * DP; }
     static constexpr bool kBf16Type = std::is_same_v<T, __nv_bfloat16>;
 
@@ -157,26 +167,23 @@ struct Kernel {
 
     __device__ uint32_t *status() const { return g.a.status ? g.a.status : &g_attention_status; }
 
-    // Waits for a phase; gives up after the budget, and at once when any wait of the CTA has given up. A try itself
-    // waits for some microseconds, so the clock is read only after many.
-    __device__ __noinline__ void wait_slow(uint64_t *bar, uint32_t parity) const {
-        volatile uint32_t *dead = &c->dead;
-        uint64_t t0 = 0;
-        for (uint32_t n = 1;; ++n) {
-            if (mbar_try_wait(bar, parity) || *dead) return;
-            if (n % 64) continue;
-            const uint64_t now = globaltimer_ns();
-            if (!t0) t0 = now;
-            if (now - t0 > g.budget) {
+    // Waits for a phase; gives up after the budget (a try waits for about a microsecond), and at once when any wait
+    // of the CTA has given up.
+    __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity) const {
+        uint32_t left = g.tries;
+        while (__builtin_expect(!mbar_try_wait_1us(bar, parity), 0)) {
+            volatile uint32_t *dead = &c->dead;
+            if (*dead) break;
+            if (--left == 0) {
                 *dead = 1;
                 atomicOr(status(), kStatusLoadTimeout);
-                return;
             }
         }
     }
-    __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity) const {
-        if (!mbar_try_wait(bar, parity)) wait_slow(bar, parity);
-    }
+
+    // A value that all lanes have, in a form that the compiler knows to be the same for all: control flow that
+    // hangs on it stays uniform, and matrix instructions take their operands without a detour per lane.
+    static __device__ __forceinline__ int same(int v) { return __reduce_or_sync(~0u, v); }
 
     // Whether some wait has given up, the same for a whole warp.
     __device__ __forceinline__ bool gave_up() const {
@@ -188,6 +195,9 @@ struct Kernel {
         const int slot = n % kRunSlots;
         wait(&c->run_full[slot], (n / kRunSlots) & 1);
         RunInfo r = c->run[slot];
+        int *fields = reinterpret_cast<int *>(&r);
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(RunInfo) / sizeof(int)); ++i) fields[i] = same(fields[i]);
         if (gave_up()) r.blocks = 0;
         if (lane == 0) mbar_arrive(&c->run_empty[slot]);
         ++n;
@@ -325,15 +335,48 @@ struct Kernel {
         drain_loads(2 * n_block);
     }
 
-    // ---- warp 11: V ----
-    __device__ void value_loop(const CUtensorMap *boxes, const CUtensorMap *lines) const {
-        int n_run = 0;
+    // ---- warp 11: queries, and V ----
+    __device__ void value_loop(const CUtensorMap *boxes, const CUtensorMap *lines, const CUtensorMap *queries) const {
+        const int each = g.shape.parts / g.a.kv_heads, tokens = g.shape.tokens_stream;
+        int n_run = 0, n_q[2] = {0, 0};
         int64_t n_block = 0;
         for (;;) {
             const RunInfo r = take_run(n_run);
-            if (!r.blocks || !load_blocks<1>(boxes, lines, r, n_block)) break;
+            if (!r.blocks) break;
+            const int head = g.each.div(r.part);
+            for (int s = 0; s <= (r.tokens > tokens); ++s) {
+                wait(&c->q_empty[s], (n_q[s] & 1) ^ 1);
+                if (gave_up()) break;
+                ++n_q[s];
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(&c->q_full[s], tokens * g.shape.heads * 128 * kHalves);
+                    for (int h = 0; h < kHalves; ++h)
+                        tma_load_4d(smem + L::kQ + s * L::kTile + h * kHalfBytes, queries, &c->q_full[s], h * 64,
+                                    (r.part - head * each) * g.shape.heads, head, r.q0 + r.t0 + s * tokens);
+                }
+                __syncwarp();
+            }
+            if (!load_blocks<1>(boxes, lines, r, n_block)) break;
         }
         drain_loads(2 * n_block + 1);
+        if (gave_up() && lane == 0)
+            for (int s = 0; s < 2; ++s)
+                if (n_q[s]) mbar_wait_bounded(&c->q_full[s], (n_q[s] - 1) & 1, g.budget / 8);
+        if (g.a.fill_tail) fill_tail();
+    }
+
+    // Zeros in the rows of no sequence.
+    __device__ void fill_tail() const {
+        const PagedAttentionArgs &a = g.a;
+        const int n = a.batch.seqs;
+        const int head = n ? plan_clamp(a.batch.starts.at(0), 0, a.rows) : static_cast<int>(a.rows);
+        const int tail = n ? plan_clamp(a.batch.starts.at(n), head, a.rows) : static_cast<int>(a.rows);
+        const int64_t rows = head + a.rows - tail, per = a.q_heads * static_cast<int64_t>(a.dim);
+        for (int64_t i = blockIdx.x * 32 + lane; i < rows * per; i += gridDim.x * 32) {
+            const int64_t k = i / per, e = i - k * per, row = k < head ? k : tail + (k - head);
+            static_cast<T *>(a.out)[row * a.o_st + e / a.dim * a.o_sh + e % a.dim] = from_f32<T>(0.f);
+            if (a.lse && e % a.dim == 0) a.lse[row * a.q_heads + e / a.dim] = -INFINITY;
+        }
     }
 
     // After a wait that ran out, loads may be in flight that nobody has waited
@@ -357,10 +400,10 @@ struct Kernel {
     // Loads the blocks of a run into the ring: K of block i is load 2 i, V is load 2 i + 1. False: a wait gave up.
     template <int PLANE>
     __device__ bool load_blocks(const CUtensorMap *boxes, const CUtensorMap *lines, const RunInfo &r, int64_t &n_block) const {
-        const int nbox = kBlockKeys / g.box, nhalf = g.pool.whole ? 1 : kHalves;
-        const int half = lane / nbox, box = lane - half * nbox;  // up to 16 boxes in each half
+        const int nbox = 1 << g.box_shift, nhalf = g.pool.whole ? 1 : kHalves;
+        const int half = lane >> g.box_shift, box = lane & (nbox - 1);  // up to 16 boxes in each half
         const bool active = half < nhalf;
-        const int head = r.part / (g.shape.parts / g.a.kv_heads), none = g.pool.none;
+        const int head = g.each.div(r.part), none = g.pool.none;
         const uint32_t at = box * (g.box / 8) * g.pool.group_bytes + half * g.pool.half_bytes;
         int key = r.key0 + box * g.box;
         bool bad = false;
@@ -408,9 +451,9 @@ struct Kernel {
                     cuts &= cuts - 1;
                     const int ck = __shfl_sync(~0u, now_key, l), ci = __shfl_sync(~0u, now, l), cs = __shfl_sync(~0u, slot, l);
                     const uint32_t to = __shfl_sync(~0u, at, l);
-                    const int from = g.pool.whole ? 0 : l / nbox, rows = g.box * (g.pool.whole ? kHalves : 1);
+                    const int from = g.pool.whole ? 0 : l >> g.box_shift, rows = g.box * (g.pool.whole ? kHalves : 1);
                     for (int e = lane; e < rows; e += 32) {
-                        const int h = e / g.box, row = e - h * g.box;
+                        const int h = e >> (7 - g.box_shift), row = e & (g.box - 1);
                         tma_load_5d(tile + to + h * g.pool.half_bytes + row / 8 * g.pool.group_bytes + row % 8 * 128, lines, bar,
                                     (from + h) * 64, cs + row, 0, 0, ck + row >= r.lo && ck + row < r.hi ? ci : none);
                     }
@@ -420,111 +463,107 @@ struct Kernel {
         return true;
     }
 
-    // ---- warp 9: matrix instructions ----
-    __device__ void mma_loop(uint32_t tmem) const {
+    // ---- warps 9, 10: matrix instructions of a stream ----
+    __device__ void mma_loop(uint32_t tmem, int s) const {
         const int ksteps = (g.a.dim + 15) / 16;
-        const uint32_t qk = mma_desc(kBf16Type, false, kBlockKeys);
+        const uint32_t qk = mma_desc(kBf16Type, false, kHalfKeys) | (g.a.scale < 0.f ? kMmaNegateA : 0u);
         const uint32_t pv = mma_desc(kBf16Type, true, ksteps * 16);
         const uint32_t base = smem_u32(smem);
         const uint32_t group = g.pool.group_bytes, halves = g.pool.half_bytes;
-        int n_run = 0, n_q[2] = {0, 0}, n_p[2] = {0, 0};
-        int64_t kv0 = 0;
+        const uint32_t to = tmem + o_at(s);
+        int n_run = 0, n_q[2] = {0, 0}, n_p = 0;
+        int kv_stage = 0, kv_phase = 0;  // of the run's first load
+        auto advance = [](int &stage, int &phase, int by) {
+            stage += by;
+            if (stage >= L::kStages) stage -= L::kStages, phase ^= 1;
+        };
         for (;;) {
             const RunInfo r = take_run(n_run);
             if (!r.blocks) break;
             const bool pair = r.tokens > g.shape.tokens_stream;
-            const int n[2] = {pair ? r.blocks : (r.blocks + 1) / 2, pair ? r.blocks : r.blocks / 2};
-            for (int t = 0; t <= pair; ++t) wait(&c->q_full[t], n_q[t]++ & 1);
-            auto scores = [&](int s, int i) {
-                const int block = pair ? i : 2 * i + s;
-                const int64_t idx = kv0 + 2 * block;
-                const int stage = static_cast<int>(idx % L::kStages);
-                wait(&c->kv_full[stage], (idx / L::kStages) & 1);
-                tmem_fence_after();
+            const int q_tile = pair ? s : 0;
+            const int n = 2 * (pair ? r.blocks : (r.blocks + 1 - s) / 2);
+            // Where the next scores' keys and the next values lie in the ring: K of a block, then its V.
+            const int step = pair ? 2 : 4;
+            int k_stage = kv_stage, k_phase = kv_phase;
+            if (!pair && s) advance(k_stage, k_phase, 2);
+            int v_stage = k_stage, v_phase = k_phase;
+            advance(v_stage, v_phase, 1);
+            wait(&c->q_full[q_tile], n_q[q_tile] & 1);
+            ++n_q[0];
+            n_q[1] += pair;
+            // Scores of the i-th half block of the stream's keys.
+            auto scores = [&](int i) {
+                if (!(i & 1)) wait(&c->kv_full[k_stage], k_phase);
                 if (elect_one()) {
-                    const uint64_t qd = smem_tile_desc(base + L::kQ + (pair ? s : 0) * L::kTile, 16, 1024);
-                    const uint64_t kd = smem_tile_desc(base + L::kKv + stage * L::kTile, 16, group);
-                    for (int e = 0; e < ksteps; ++e)
-                        mma_ss(tmem + s_at(s), qd + ((e >> 2) * kHalfBytes + (e & 3) * 32) / 16,
-                               kd + ((e >> 2) * halves + (e & 3) * 32) / 16, qk, e > 0);
-                    if (!pair || s == 1) mma_commit(&c->kv_empty[stage]);
-                    if (pair ? i + 1 == n[s] : block + 1 == r.blocks) mma_commit(&c->q_empty[pair ? s : 0]);
-                    mma_commit(&c->s_full[s]);
-                }
-                __syncwarp();
-            };
-            auto values = [&](int s, int i) {
-                const int block = pair ? i : 2 * i + s;
-                const int64_t idx = kv0 + 2 * block + 1;
-                const int stage = static_cast<int>(idx % L::kStages);
-                wait(&c->kv_full[stage], (idx / L::kStages) & 1);
-                wait(&c->p_full[s], n_p[s]++ & 1);
-                tmem_fence_after();
-                if (elect_one()) {
-                    const uint64_t vd = smem_tile_desc(base + L::kKv + stage * L::kTile, halves, group);
+                    const uint64_t qd = smem_tile_desc(base + L::kQ + q_tile * L::kTile, 16, 1024);
+                    const uint64_t kd = smem_tile_desc(base + L::kKv + k_stage * L::kTile + (i & 1) * 8 * group, 16, group);
+                    const uint32_t at = tmem + s_at(s, i & 1);
 #pragma unroll
-                    for (int e = 0; e < kBlockKeys / 16; ++e)
-                        mma_ts(tmem + o_at(s), tmem + s_at(s) + e * 8, vd + e * (group / 8), pv, i > 0 || e > 0);
-                    if (!pair || s == 1) mma_commit(&c->kv_empty[stage]);
-                    if (i + 1 == n[s]) mma_commit(&c->o_full[s]);
+                    for (int e = 0; e < DP / 16; ++e)
+                        if (e < ksteps)
+                            mma_ss(at, qd + ((e >> 2) * kHalfBytes + (e & 3) * 32) / 16, kd + ((e >> 2) * halves + (e & 3) * 32) / 16,
+                                   qk, e > 0);
+                    mma_commit(&c->s_full[s][i & 1]);
+                    if (i & 1) {
+                        // two arrivals free a block or a tile of queries: both streams', or one's if the other has no use for it
+                        mma_commit(&c->kv_empty[k_stage]);
+                        if (!pair) mma_commit(&c->kv_empty[k_stage]);
+                        if (i + 1 == n) {
+                            mma_commit(&c->q_empty[q_tile]);
+                            if (pair) mma_commit(&c->q_empty[q_tile]);
+                        }
+                    }
                 }
                 __syncwarp();
+                if (i & 1) advance(k_stage, k_phase, step);
             };
-            scores(0, 0);
-            if (n[1]) scores(1, 0);
-            for (int i = 0; i < n[0]; ++i) {
-                for (int s = 0; s < 2; ++s) {
-                    if (i >= n[s]) continue;
-                    values(s, i);
-                    if (i + 1 < n[s]) scores(s, i + 1);
-                }
+            if (n) {
+                tmem_fence_after();
+                scores(0);
+                scores(1);
+            } else if (lane == 0) {
+                mbar_arrive(&c->q_empty[q_tile]);
             }
-            kv0 += 2 * r.blocks;
-        }
-        if (gave_up()) {
-            // instructions may be in flight whose end nobody has seen: tensor memory stays ours until then
-            if (elect_one()) {
-                mma_commit(&c->drain);
-                mbar_wait_bounded(&c->drain, 0, g.budget);
-            }
-            __syncwarp();
-        }
-    }
-
-    // ---- warp 10: queries ----
-    __device__ void query_loop(const CUtensorMap *queries) const {
-        const PagedAttentionArgs &a = g.a;
-        const int each = g.shape.parts / a.kv_heads, tokens = g.shape.tokens_stream;
-        int n_run = 0, n_q[2] = {0, 0};
-        for (;;) {
-            const RunInfo r = take_run(n_run);
-            if (!r.blocks) break;
-            for (int s = 0; s <= (r.tokens > tokens); ++s) {
-                wait(&c->q_empty[s], (n_q[s]++ & 1) ^ 1);
-                if (!gave_up() && elect_one()) {
-                    mbar_arrive_expect_tx(&c->q_full[s], tokens * g.shape.heads * 128 * kHalves);
-                    for (int h = 0; h < kHalves; ++h)
-                        tma_load_4d(smem + L::kQ + s * L::kTile + h * kHalfBytes, queries, &c->q_full[s], h * 64,
-                                    r.part % each * g.shape.heads, r.part / each, r.q0 + r.t0 + s * tokens);
+            for (int i = 0; i < n; ++i) {
+                // output += weights times values
+                if (!(i & 1)) wait(&c->kv_full[v_stage], v_phase);
+                wait(&c->p_full[s][i & 1], n_p++ >> 1 & 1);
+                tmem_fence_after();
+                if (elect_one()) {
+                    const uint64_t vd = smem_tile_desc(base + L::kKv + v_stage * L::kTile + (i & 1) * 8 * group, halves, group);
+                    const uint32_t from = tmem + s_at(s, i & 1);
+#pragma unroll
+                    for (int e = 0; e < kHalfKeys / 16; ++e) mma_ts(to, from + e * 8, vd + e * (group / 8), pv, i > 0 || e > 0);
+                    mma_commit(&c->o_step[s]);
+                    if (i & 1) {
+                        mma_commit(&c->kv_empty[v_stage]);
+                        if (!pair) mma_commit(&c->kv_empty[v_stage]);
+                        if (i + 1 == n) mma_commit(&c->o_full[s]);
+                    }
                 }
                 __syncwarp();
+                if (i & 1) advance(v_stage, v_phase, step);
+                if (pair) {
+                    if (i + 2 < n) scores(i + 2);
+                } else if ((i & 1) && i + 1 < n) {
+                    // K of a stream's next block only after V of this one is free: the two streams would otherwise hold
+                    // four tiles of the ring, and there would be little room to load ahead
+                    scores(i + 1);
+                    scores(i + 2);
+                }
             }
+            int ahead = 2 * r.blocks % (2 * L::kStages);
+            if (ahead >= L::kStages) ahead -= L::kStages, kv_phase ^= 1;
+            advance(kv_stage, kv_phase, ahead);
         }
-        if (gave_up() && lane == 0)  // as drain_loads
-            for (int s = 0; s < 2; ++s)
-                if (n_q[s]) mbar_wait_bounded(&c->q_full[s], (n_q[s] - 1) & 1, g.budget / 8);
-        if (a.fill_tail) {
-            // rows of no sequence
-            const int n = a.batch.seqs;
-            const int head = n ? plan_clamp(a.batch.starts.at(0), 0, a.rows) : static_cast<int>(a.rows);
-            const int tail = n ? plan_clamp(a.batch.starts.at(n), head, a.rows) : static_cast<int>(a.rows);
-            const int64_t rows = head + a.rows - tail, per = a.q_heads * static_cast<int64_t>(a.dim);
-            for (int64_t i = blockIdx.x * 32 + lane; i < rows * per; i += gridDim.x * 32) {
-                const int64_t k = i / per, e = i - k * per, row = k < head ? k : tail + (k - head);
-                static_cast<T *>(a.out)[row * a.o_st + e / a.dim * a.o_sh + e % a.dim] = from_f32<T>(0.f);
-                if (a.lse && e % a.dim == 0) a.lse[row * a.q_heads + e / a.dim] = -INFINITY;
-            }
+        // What the last instructions arrive on is this CTA's memory, and they use tensor memory: both stay until they
+        // are done.
+        if (elect_one()) {
+            mma_commit(&c->drain[s]);
+            mbar_wait_bounded(&c->drain[s], 0, g.budget);
         }
+        __syncwarp();
     }
 
     // ---- warps 0-7: softmax ----
@@ -535,33 +574,63 @@ struct Kernel {
         return r;
     }
 
-    // Replaces the scores of columns outside [lo, hi) and on boxes that are not there.
-    __device__ __forceinline__ void mask_scores(uint32_t (&x)[4][32], int lo, int hi, uint32_t boxes) const {
-        const int shift = __ffs(g.box) - 1;
+    // Replaces the scores of columns outside [lo, hi) and on boxes that are not there; the first column is key
+    // `at` of its block.
+    __device__ __forceinline__ void mask_scores(uint32_t (&x)[2][32], int lo, int hi, int at, uint32_t boxes) const {
+        const int shift = 7 - g.box_shift;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
             const int up = hi - j * 32, down = lo - j * 32;
             uint32_t seen = up >= 32 ? ~0u : up <= 0 ? 0u : (1u << up) - 1;
             if (down > 0) seen = down >= 32 ? 0u : seen & (~0u << down);
             if (boxes != ~0u)
-                for (int e = 0; e < 32; ++e) seen &= ~((~boxes >> ((j * 32 + e) >> shift) & 1u) << e);
+                for (int e = 0; e < 32; ++e) seen &= ~((~boxes >> ((at + j * 32 + e) >> shift) & 1u) << e);
 #pragma unroll
             for (int e = 0; e < 32; ++e)
                 if (!(seen >> e & 1u)) x[j][e] = 0xff800000u;
         }
     }
 
-    // The largest of a row's 128 scores, by four chains.
-    static __device__ __forceinline__ float largest(const uint32_t (&x)[4][32]) {
+    // The largest of a row's 64 scores, by four chains; NaN if one is.
+    static __device__ __forceinline__ float largest(const uint32_t (&x)[2][32]) {
         float t[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            t[j] = fmaxf(__uint_as_float(x[j][0]), __uint_as_float(x[j][1]));
+            const uint32_t *y = x[j / 2] + j % 2 * 16;
+            t[j] = max_nan(__uint_as_float(y[0]), __uint_as_float(y[1]));
 #pragma unroll
-            for (int e = 2; e < 32; e += 2)
-                t[j] = fmaxf(fmaxf(t[j], __uint_as_float(x[j][e])), __uint_as_float(x[j][e + 1]));
+            for (int e = 2; e < 16; e += 2) t[j] = max_nan(t[j], __uint_as_float(y[e]), __uint_as_float(y[e + 1]));
         }
-        return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        return max_nan(max_nan(t[0], t[1]), t[2], t[3]);
+    }
+
+    // Scores to weights: x[j] = 2^(x[j] * times + less), and the weights in 16 bits to tensor memory. Some
+    // exponentials go to the FMA pipes: the special function unit alone takes 512 cycles for a warp's rows.
+    static __device__ __forceinline__ void weigh(uint32_t (&x)[32], float times, float less, uint32_t to) {
+        const Pair times2 = make_pair(times, times), less2 = make_pair(less, less);
+        uint32_t p[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float u, v;
+            split(fma2(make_pair(x[2 * e], x[2 * e + 1]), times2, less2), u, v);
+            if (e * kFmaPairs % 16 < kFmaPairs) {
+                split(exp2_fma(u, v), u, v);
+            } else {
+                u = exp2_approx(u);
+                v = exp2_approx(v);
+            }
+            p[e] = pack(u, v);
+            x[2 * e] = __float_as_uint(u);
+            x[2 * e + 1] = __float_as_uint(v);
+        }
+        tmem_st16(to, p);
+    }
+
+    __device__ __forceinline__ void hand_over(uint64_t *bar) const {
+        tmem_wait_st();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
     }
 
     __device__ void softmax_loop(uint32_t tmem, int s) const {
@@ -571,16 +640,17 @@ struct Kernel {
         const int row_token = row / shape.heads, row_head = row - row_token * shape.heads;
         const int each = shape.parts / a.kv_heads;
         const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-        const uint32_t ts = tmem + s_at(s) + lanes, to = tmem + o_at(s) + lanes;
+        const uint32_t to = tmem + o_at(s) + lanes;
         const float scale = g.scale_log2;
-        int n_run = 0, n_s = 0, n_o = 0, n_block = 0, n_join = 0;
+        int n_run = 0, n_s = 0, n_o = 0, n_block = 0, n_join = 0, n_turn = 0;
         for (;;) {
             const RunInfo r = take_run(n_run);
             if (!r.blocks) break;
             const bool pair = r.tokens > shape.tokens_stream;
             const int steps = pair ? r.blocks : (r.blocks + 1 - s) / 2;
             const int token = pair ? s * shape.tokens_stream + row_token : row_token;  // of the tile
-            const int head_group = r.part % each * shape.heads + row_head;
+            const int kv_head = g.each.div(r.part);
+            const int head_group = (r.part - kv_head * each) * shape.heads + row_head;
             const bool live = row_token < shape.tokens_stream && token < r.tokens && head_group < g.group;
             const bool work = __any_sync(~0u, live);
             int lo = 0, hi = 1 << 30;  // keys that the row sees
@@ -592,91 +662,85 @@ struct Kernel {
             // keys that every row of the warp sees: blocks inside need no mask
             const int all_lo = __reduce_max_sync(~0u, lo), all_hi = __reduce_min_sync(~0u, hi);
             bool huge = false;  // some row's m is too large for one rounding (below)
-            float m = -INFINITY, ref = 0.f, sum = 0.f;  // m = ref * scale
-            for (int i = 0; i < steps; ++i) {
-                const int block = pair ? i : 2 * i + s;
-                const int key0 = r.key0 + block * kBlockKeys;
-                wait(&c->s_full[s], n_s++ & 1);
+            float m = -INFINITY, ref = 0.f, less = 0.f, sum = 0.f;  // m = ref * scale, less = -m
+            for (int i = 0; i < 2 * steps; ++i) {
+                const int half = i & 1, block = pair ? i / 2 : i / 2 * 2 + s;
+                const int key0 = r.key0 + block * kBlockKeys + half * kHalfKeys;
+                const uint32_t ts = tmem + s_at(s, half) + lanes;
+                wait(&c->s_full[s][half], n_s++ >> 1 & 1);
                 tmem_fence_after();
                 if (work) {
-                    uint32_t x[4][32];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) tmem_ld32(ts + j * 32, x[j]);
+                    uint32_t x[2][32];
+                    tmem_ld32(ts, x[0]);
+                    tmem_ld32(ts + 32, x[1]);
                     const uint32_t boxes = c->mask[(n_block + block) % kMaskSlots];
                     tmem_wait_ld();
-                    if (g.negate) {
-#pragma unroll
-                        for (int j = 0; j < 128; ++j) x[j / 32][j % 32] ^= 0x80000000u;
-                    }
-                    if (all_hi < key0 + kBlockKeys || all_lo > key0 || boxes != ~0u) mask_scores(x, lo - key0, hi - key0, boxes);
+                    if (__builtin_expect(all_hi < key0 + kHalfKeys || all_lo > key0 || boxes != ~0u, 0))
+                        mask_scores(x, lo - key0, hi - key0, half * kHalfKeys, boxes);
                     const float top = largest(x);
                     // m, a reference in units of log2
                     const float next = top * scale;
-                    const bool move = next > m + kRescale;
-                    const float was = m;
-                    const bool moves = __any_sync(~0u, move && live);
-                    if (moves) {
+                    const bool move = !(next <= m + kRescale);  // NaN moves it too
+                    if (__builtin_expect(__any_sync(~0u, move && live), 0)) {
+                        const float was = m;
                         if (move) m = next, ref = top;
+                        // the weights of a row with a NaN or an infinite score are NaN; nothing seen yet: zero
+                        less = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m;
+                        // x * scale - m is off by what m was rounded by, the same for the whole row, so it cancels;
+                        // where it could pass 1 (the lowest value of a type as a score) the reference comes off first.
                         huge = __any_sync(~0u, live && fabsf(m) > 0x1p24f && m != -INFINITY);
+                        if (i > 0) {
+                            const float keep = move ? exp2_approx(was - m) : 1.f;
+                            sum *= keep;
+                            // The output so far is complete when the last half block's weights have been used (the
+                            // one before has: its buffer holds these scores). n_s counts this half block already.
+                            wait(&c->o_step[s], n_s & 1);
+                            tmem_fence_after();
+#pragma unroll 1
+                            for (int j = 0; j < a.dim; j += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(to + j, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                                tmem_st16(to + j, o);
+                            }
+                        }
                     }
-                    float less = m == -INFINITY ? 0.f : -m, times = scale;
-                    // x * scale - m is off by what m was rounded by, the same for the whole row, so it cancels;
-                    // where it could pass 1 (the lowest value of a type as a score) the reference comes off first.
-                    if (huge) {
+                    float times = scale, minus = less;
+                    if (__builtin_expect(huge, 0)) {
                         const float off = m == -INFINITY ? 0.f : ref;
 #pragma unroll
-                        for (int j = 0; j < 128; ++j)
+                        for (int j = 0; j < kHalfKeys; ++j)
                             x[j / 32][j % 32] = __float_as_uint((__uint_as_float(x[j / 32][j % 32]) - off) * scale);
-                        less = 0.f;
+                        minus = less * 0.f;
                         times = 1.f;
                     }
-                    const Pair times2 = make_pair(times, times), less2 = make_pair(less, less);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float u, v;
-                            split(fma2(make_pair(x[j][2 * e], x[j][2 * e + 1]), times2, less2), u, v);
-                            u = exp2_approx(u);
-                            v = exp2_approx(v);
-                            p[e] = pack(u, v);
-                            x[j][2 * e] = __float_as_uint(u);
-                            x[j][2 * e + 1] = __float_as_uint(v);
-                        }
-                        tmem_st16(ts + j * 16, p);
-                    }
-                    if (i > 0 && moves) {
-                        const float keep = move ? exp2_approx(was - m) : 1.f;
-                        sum *= keep;
-                        for (int j = 0; j < a.dim; j += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(to + j, o);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tmem_st16(to + j, o);
-                        }
-                    }
-                    tmem_wait_st();
-                    tmem_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&c->p_full[s]);
+                    if (pair) wait(&c->turn[s][warp], (n_turn++ & 1) ^ (s == 0));
+                    weigh(x[0], times, minus, ts);
+                    weigh(x[1], times, minus, ts + 16);
+                    if (pair && lane == 0) mbar_arrive(&c->turn[s ^ 1][warp]);
+                    hand_over(&c->p_full[s][half]);
                     // the sum is taken while the tensor core has the weights
                     Pair add[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        add[j] = make_pair(x[j][0], x[j][1]);
+                        const uint32_t *y = x[j / 2] + j % 2 * 16;
+                        add[j] = make_pair(y[0], y[1]);
 #pragma unroll
-                        for (int e = 2; e < 32; e += 2) add[j] = add2(add[j], make_pair(x[j][e], x[j][e + 1]));
+                        for (int e = 2; e < 16; e += 2) add[j] = add2(add[j], make_pair(y[e], y[e + 1]));
                     }
                     float s0, s1;
                     split(add2(add2(add[0], add[1]), add2(add[2], add[3])), s0, s1);
                     sum += s0 + s1;
                 } else {
+                    if (pair) wait(&c->turn[s][warp], (n_turn++ & 1) ^ (s == 0));
                     tmem_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&c->p_full[s]);
+                    if (lane == 0) {
+                        if (pair) mbar_arrive(&c->turn[s ^ 1][warp]);
+                        mbar_arrive(&c->p_full[s][half]);
+                    }
                 }
             }
             n_block += r.blocks;
@@ -686,6 +750,7 @@ struct Kernel {
             }
             if (!pair) {
                 if (s == 1) {
+                    if (m == -INFINITY) sum = 0.f;
                     c->join[row][0] = m;
                     c->join[row][1] = sum;
                     tmem_fence_before();
@@ -695,6 +760,7 @@ struct Kernel {
                     wait(&c->join_full, n_join & 1);
                 }
             }
+            if (m == -INFINITY) sum = 0.f;  // no score: the weights are what 2^x gives at the least
             if (work && (pair || s == 0)) {
                 tmem_fence_after();
                 float k0 = 1.f, k1 = 0.f;
@@ -707,7 +773,7 @@ struct Kernel {
                     m = all;
                 }
                 const int64_t q_row = r.q0 + r.t0 + token;
-                const int head = r.part / each * g.group + head_group;
+                const int head = kv_head * g.group + head_group;
                 const int slot_row = (pair ? s * kStreamRows : 0) + row;
                 char *slot = static_cast<char *>(a.workspace) + shared_bytes(g.ctas) + (2 * blockIdx.x + r.slot) * slot_bytes(DP);
                 T *out = static_cast<T *>(a.out) + q_row * a.o_st + head * a.o_sh;
@@ -716,27 +782,23 @@ struct Kernel {
                     k0 *= inv;
                     k1 *= inv;
                 }
-                for (int j = 0; j < a.dim; j += 16) {
-                    uint32_t o[16];
-                    tmem_ld16(to + j, o);
+#pragma unroll 1
+                for (int j = 0; j < a.dim; j += 32) {
+                    uint32_t o[32], o1[32];
+                    tmem_ld32(to + j, o);
+                    if (both) tmem_ld32(tmem + o_at(1) + lanes + j, o1);
                     tmem_wait_ld();
-                    float f[16];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) f[e] = __uint_as_float(o[e]) * k0;
-                    if (both) {
-                        tmem_ld16(tmem + o_at(1) + lanes + j, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) f[e] = fmaf(__uint_as_float(o[e]), k1, f[e]);
-                    }
-                    if (sum == 0.f) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) f[e] = 0.f;
-                    }
                     if (!live) continue;
+                    float f[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        f[e] = __uint_as_float(o[e]) * k0;
+                        if (both) f[e] = fmaf(__uint_as_float(o1[e]), k1, f[e]);
+                        if (sum == 0.f) f[e] = 0.f;
+                    }
                     if (r.slot < 0) {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 8)
+                        for (int e = 0; e < 32; e += 8)
                             if (j + e < a.dim)
                                 *reinterpret_cast<uint4 *>(out + j + e) =
                                     make_uint4(pack(f[e], f[e + 1]), pack(f[e + 2], f[e + 3]), pack(f[e + 4], f[e + 5]),
@@ -744,7 +806,7 @@ struct Kernel {
                     } else {
                         float *o32 = reinterpret_cast<float *>(slot) + slot_row * DP + j;
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4 *>(o32 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(o32 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
                     }
                 }
                 if (live && r.slot >= 0)
@@ -782,18 +844,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         c->dead = 0;
         for (int i = 0; i < K::L::kStages; ++i) {
             mbar_init(&c->kv_full[i], 1);
-            mbar_init(&c->kv_empty[i], 1);
+            mbar_init(&c->kv_empty[i], 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&c->q_full[i], 1);
-            mbar_init(&c->q_empty[i], 1);
-            mbar_init(&c->s_full[i], 1);
-            mbar_init(&c->p_full[i], 4);
+            mbar_init(&c->q_empty[i], 2);
+            for (int j = 0; j < 4; ++j) mbar_init(&c->turn[i][j], 1);
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&c->s_full[i][j], 1);
+                mbar_init(&c->p_full[i][j], 4);
+            }
+            mbar_init(&c->o_step[i], 1);
             mbar_init(&c->o_full[i], 1);
         }
         mbar_init(&c->join_full, 4);
         mbar_init(&c->join_empty, 4);
-        mbar_init(&c->drain, 1);
+        mbar_init(&c->drain[0], 1);
+        mbar_init(&c->drain[1], 1);
         for (int i = 0; i < kRunSlots; ++i) {
             mbar_init(&c->run_full[i], 1);
             mbar_init(&c->run_empty[i], 11);  // warps 0-7 and 9-11
@@ -809,13 +876,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = c->tmem;
+    const uint32_t tmem = K::same(c->tmem);
     pdl_launch();
-    if (warp < 8) k.softmax_loop(tmem, warp >> 2);
-    else if (warp == 8) k.plan_loop(&boxes, &lines);
-    else if (warp == 9) k.mma_loop(tmem);
-    else if (warp == 10) k.query_loop(&queries);
-    else k.value_loop(&boxes, &lines);
+    if (warp < 8) {
+        take_registers<kRegsSoftmax>();
+        k.softmax_loop(tmem, warp >> 2);
+    } else {
+        give_registers<kRegsOther>();
+        if (warp == 8) k.plan_loop(&boxes, &lines);
+        else if (warp < 11) k.mma_loop(tmem, warp - 9);
+        else k.value_loop(&boxes, &lines, &queries);
+    }
     tmem_fence_before();
     __syncthreads();
     if (warp == 9) tmem_free(tmem, 512);
@@ -948,7 +1019,10 @@ int launch(KernelArgs &g, int dtype, int device, bool join, cudaStream_t st) {
     cudaError_t e = cudaSuccess;
     if (device > 63 || !(configured.load(std::memory_order_acquire) >> device & 1)) {
         e = cudaFuncSetAttribute(paged_attention_kernel<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaFuncAttributes attr;
+        if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, paged_attention_kernel<DP, T>);
         if (e != cudaSuccess) return static_cast<int>(e);
+        if (attr.numRegs != kRegsLaunch) return cudaErrorLaunchOutOfResources;  // the split above would not add up
         if (device <= 63) configured.fetch_or(1ull << device, std::memory_order_release);
     }
     paged_attention_kernel<DP, T><<<g.ctas, kThreads, smem, st>>>(g, boxes, lines, queries);
@@ -995,16 +1069,19 @@ int paged_attention(const PagedAttentionArgs &a, int dtype, int device, void *st
     g.shape.tokens = plan_clamp(tokens, 0, kMostTokens);
     // a scale of zero would make NaN of a masked score; this one gives every seen score the same weight
     g.scale_log2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-30f);
-    g.negate = a.scale < 0.f;
     g.box = a.batch.page_tokens & -a.batch.page_tokens;
     if (g.box > kBlockKeys) g.box = kBlockKeys;
+    g.box_shift = 0;
+    while (g.box << g.box_shift < kBlockKeys) ++g.box_shift;
     g.page_tokens = FastDiv(static_cast<uint32_t>(a.batch.page_tokens));
+    g.each = FastDiv(static_cast<uint32_t>(g.shape.parts / a.kv_heads));
     g.pool = PoolView();
     g.pool.whole = a.dim % 64 == 0;
     const int halves = a.dim <= 64 ? 1 : 2, tile_half = kStreamRows * 128;
     g.pool.group_bytes = g.pool.whole ? 1024 * halves : 1024;
     g.pool.half_bytes = g.pool.whole ? 1024 : tile_half;
     g.budget = wait_budget_ns();
+    g.tries = static_cast<uint32_t>(plan_clamp(static_cast<int64_t>(g.budget / 1000), 1, 0x7fffffff));
     g.ctas = plan_ctas(a, g.shape, sm_count(device));
     if (!a.workspace || a.workspace_bytes < shared_bytes(g.ctas) + 2 * g.ctas * slot_bytes(a.dim <= 64 ? 64 : 128))
         return cudaErrorInvalidValue;

@@ -94,6 +94,8 @@ __host__ __device__ constexpr uint32_t mma_desc(bool bf16, bool b_mn, int n) {
            (128u >> 4) << 24;
 }
 
+constexpr uint32_t kMmaNegateA = 1u << 13;
+
 // D (tensor memory) = A B^T (+ D), K = 16; A from shared memory.
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
     asm volatile(
@@ -137,8 +139,31 @@ __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap *map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
 
+// A try that is suspended for a microsecond at most.
+__device__ __forceinline__ bool mbar_try_wait_1us(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// ---- registers of a warpgroup ----
+template <int N>
+__device__ __forceinline__ void take_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void give_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // ---- programmatic dependent launch ----
@@ -177,6 +202,35 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// 2^x of two values on the FMA pipes, for x <= 127; below -126 it is 2^-126.
+// x = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 leaves n in the low
+// bits), 2^f by a polynomial of degree 5 fitted for the least relative error
+// (2.3e-7 in 32-bit arithmetic), and n goes into the exponent.
+__device__ __forceinline__ Pair exp2_fma(float lo, float hi) {
+    const Pair x = make_pair(max_nan(lo, -126.f), max_nan(hi, -126.f));
+    const Pair t = add2(x, make_pair(12582912.f, 12582912.f));
+    const Pair n = add2(t, make_pair(-12582912.f, -12582912.f));
+    const Pair f = fma2(n, make_pair(-1.f, -1.f), x);
+    constexpr float c[6] = {0x1.000002p+0f, 0x1.62e428p-1f, 0x1.ebf918p-3f, 0x1.c6b6e4p-5f, 0x1.3d0c52p-7f, 0x1.5c08e4p-10f};
+    Pair p = make_pair(c[5], c[5]);
+#pragma unroll
+    for (int i = 4; i >= 0; --i) p = fma2(p, f, make_pair(c[i], c[i]));
+    float p0, p1, t0, t1;
+    split(p, p0, p1);
+    split(t, t0, t1);
+    return make_pair(__float_as_uint(p0) + (__float_as_uint(t0) << 23), __float_as_uint(p1) + (__float_as_uint(t1) << 23));
 }
 
 }  // namespace kern
