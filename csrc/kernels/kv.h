@@ -115,8 +115,8 @@ struct PagedAttentionArgs {
     size_t workspace_bytes = 0;
     uint32_t *status = nullptr;
 };
-// Bytes of workspace that a call of these sizes needs (0: none).
-size_t paged_attention_workspace(int64_t rows, int q_heads, int kv_heads, int dim, int seqs, int device);
+// Bytes of workspace that a call needs (its contents do not matter), 16-byte aligned.
+size_t paged_attention_workspace(int dim, int device);
 int paged_attention(const PagedAttentionArgs &a, int dtype, int device, void *stream);
 
 }  // namespace kern

@@ -77,7 +77,11 @@ struct RunInfo {
 template <int DP>
 struct Layout {
     static constexpr int kTile = kStreamRows * DP * 2;  // 128 rows of DP 16-bit elements
-    static constexpr int kStages = DP == 128 ? 5 : 10;
+    // Tiles of K and of V. A wait tells a tile's phase from the next one only, so whoever waits for a tile's n-th use
+    // must have seen the one before: K and V are rings of their own, each filled by one warp, and both streams go
+    // through every tile, a stream that has no use for one passes it.
+    static constexpr int kKeys = DP == 128 ? 2 : 4, kValues = DP == 128 ? 3 : 6;
+    static constexpr int kStages = kKeys + kValues;
     static constexpr int kQ = 0;
     static constexpr int kKv = 2 * kTile;
     static constexpr int kControl = kKv + kStages * kTile;
@@ -332,7 +336,7 @@ struct Kernel {
             mbar_arrive(&c->run_full[slot]);
             static_cast<Shared *>(g.a.workspace)[blockIdx.x] = mine;
         }
-        drain_loads(2 * n_block);
+        drain_loads<0>(n_block);
     }
 
     // ---- warp 11: queries, and V ----
@@ -358,7 +362,7 @@ struct Kernel {
             }
             if (!load_blocks<1>(boxes, lines, r, n_block)) break;
         }
-        drain_loads(2 * n_block + 1);
+        drain_loads<1>(n_block);
         if (gave_up() && lane == 0)
             for (int s = 0; s < 2; ++s)
                 if (n_q[s]) mbar_wait_bounded(&c->q_full[s], (n_q[s] - 1) & 1, g.budget / 8);
@@ -379,13 +383,18 @@ struct Kernel {
         }
     }
 
+    static constexpr int ring(int plane) { return plane ? L::kValues : L::kKeys; }
+    static constexpr int ring_at(int plane) { return plane ? L::kKeys : 0; }
+
     // After a wait that ran out, loads may be in flight that nobody has waited
     // for: shared memory stays ours until they have landed. `next`: the
     // warp's next load.
+    template <int PLANE>
     __device__ void drain_loads(int64_t next) const {
+        constexpr int R = ring(PLANE);
         if (!gave_up() || lane) return;
-        for (int64_t i = next - 2; i >= 0 && i >= next - 2 * L::kStages; i -= 2)
-            mbar_wait_bounded(&c->kv_full[i % L::kStages], (i / L::kStages) & 1, g.budget / 8);
+        for (int64_t i = next - 1; i >= 0 && i >= next - R; --i)
+            mbar_wait_bounded(&c->kv_full[ring_at(PLANE) + i % R], (i / R) & 1, g.budget / 8);
     }
 
     // The index of the page of key `key` on, g.pool.none where nobody sees the box or there is no page.
@@ -397,7 +406,7 @@ struct Kernel {
         return *bad ? g.pool.none : static_cast<int>(page) * g.pool.page + plane * g.pool.plane + head * g.pool.head;
     }
 
-    // Loads the blocks of a run into the ring: K of block i is load 2 i, V is load 2 i + 1. False: a wait gave up.
+    // Loads K or V of a run's blocks into its ring. False: a wait gave up.
     template <int PLANE>
     __device__ bool load_blocks(const CUtensorMap *boxes, const CUtensorMap *lines, const RunInfo &r, int64_t &n_block) const {
         const int nbox = 1 << g.box_shift, nhalf = g.pool.whole ? 1 : kHalves;
@@ -416,9 +425,8 @@ struct Kernel {
             bad = false;
             if (i + 1 < r.blocks && active) index = place(r, head, PLANE, key, &bad);  // in flight while this block is loaded
             const int slot = now_key - g.page_tokens.div(now_key) * g.a.batch.page_tokens;
-            const int64_t n = 2 * n_block + PLANE;
-            const int stage = static_cast<int>(n % L::kStages);
-            wait(&c->kv_empty[stage], ((n / L::kStages) & 1) ^ 1);
+            const int stage = ring_at(PLANE) + static_cast<int>(n_block % ring(PLANE));
+            wait(&c->kv_empty[stage], ((n_block / ring(PLANE)) & 1) ^ 1);
             if (gave_up()) return false;
             char *tile = smem + L::kKv + stage * L::kTile;
             uint64_t *bar = &c->kv_full[stage];
@@ -472,29 +480,40 @@ struct Kernel {
         const uint32_t group = g.pool.group_bytes, halves = g.pool.half_bytes;
         const uint32_t to = tmem + o_at(s);
         int n_run = 0, n_q[2] = {0, 0}, n_p = 0;
-        int kv_stage = 0, kv_phase = 0;  // of the run's first load
-        auto advance = [](int &stage, int &phase, int by) {
-            stage += by;
-            if (stage >= L::kStages) stage -= L::kStages, phase ^= 1;
+        int k_stage = 0, k_phase = 0, v_stage = L::kKeys, v_phase = 0;  // of the next tile
+        auto next_k = [&] {
+            if (++k_stage == L::kKeys) k_stage = 0, k_phase ^= 1;
+        };
+        auto next_v = [&] {
+            if (++v_stage == L::kStages) v_stage = L::kKeys, v_phase ^= 1;
+        };
+        auto pass_k = [&] {
+            wait(&c->kv_full[k_stage], k_phase);
+            if (lane == 0) mbar_arrive(&c->kv_empty[k_stage]);
+            next_k();
+        };
+        auto pass_v = [&] {
+            wait(&c->kv_full[v_stage], v_phase);
+            if (lane == 0) mbar_arrive(&c->kv_empty[v_stage]);
+            next_v();
         };
         for (;;) {
             const RunInfo r = take_run(n_run);
             if (!r.blocks) break;
             const bool pair = r.tokens > g.shape.tokens_stream;
             const int q_tile = pair ? s : 0;
-            const int n = 2 * (pair ? r.blocks : (r.blocks + 1 - s) / 2);
-            // Where the next scores' keys and the next values lie in the ring: K of a block, then its V.
-            const int step = pair ? 2 : 4;
-            int k_stage = kv_stage, k_phase = kv_phase;
-            if (!pair && s) advance(k_stage, k_phase, 2);
-            int v_stage = k_stage, v_phase = k_phase;
-            advance(v_stage, v_phase, 1);
-            wait(&c->q_full[q_tile], n_q[q_tile] & 1);
-            ++n_q[0];
-            n_q[1] += pair;
+            const int n = 2 * (pair ? r.blocks : (r.blocks + 1 - s) / 2);  // half blocks
+            // With the same rows in both streams, blocks 2 t and 2 t + 1 are taken together, one by each stream.
+            const bool before = !pair && s == 1;
+            wait(&c->q_full[0], n_q[0]++ & 1);
+            if (pair && s == 1) wait(&c->q_full[1], n_q[1]++ & 1);
+            tmem_fence_after();
             // Scores of the i-th half block of the stream's keys.
             auto scores = [&](int i) {
-                if (!(i & 1)) wait(&c->kv_full[k_stage], k_phase);
+                if (!(i & 1)) {
+                    if (before) pass_k();
+                    wait(&c->kv_full[k_stage], k_phase);
+                }
                 if (elect_one()) {
                     const uint64_t qd = smem_tile_desc(base + L::kQ + q_tile * L::kTile, 16, 1024);
                     const uint64_t kd = smem_tile_desc(base + L::kKv + k_stage * L::kTile + (i & 1) * 8 * group, 16, group);
@@ -506,28 +525,27 @@ struct Kernel {
                                    qk, e > 0);
                     mma_commit(&c->s_full[s][i & 1]);
                     if (i & 1) {
-                        // two arrivals free a block or a tile of queries: both streams', or one's if the other has no use for it
                         mma_commit(&c->kv_empty[k_stage]);
-                        if (!pair) mma_commit(&c->kv_empty[k_stage]);
-                        if (i + 1 == n) {
-                            mma_commit(&c->q_empty[q_tile]);
-                            if (pair) mma_commit(&c->q_empty[q_tile]);
-                        }
+                        if (i + 1 == n) mma_commit(&c->q_empty[q_tile]);
                     }
                 }
                 __syncwarp();
-                if (i & 1) advance(k_stage, k_phase, step);
+                if (i & 1) {
+                    next_k();
+                    if (!pair && s == 0 && i < r.blocks) pass_k();  // block i, the other stream's
+                }
             };
+            if (s == 1 && (pair || !n) && lane == 0) mbar_arrive(&c->q_empty[0]);  // no use for the first tile: passed
             if (n) {
-                tmem_fence_after();
                 scores(0);
                 scores(1);
-            } else if (lane == 0) {
-                mbar_arrive(&c->q_empty[q_tile]);
             }
             for (int i = 0; i < n; ++i) {
                 // output += weights times values
-                if (!(i & 1)) wait(&c->kv_full[v_stage], v_phase);
+                if (!(i & 1)) {
+                    if (before) pass_v();
+                    wait(&c->kv_full[v_stage], v_phase);
+                }
                 wait(&c->p_full[s][i & 1], n_p++ >> 1 & 1);
                 tmem_fence_after();
                 if (elect_one()) {
@@ -538,24 +556,27 @@ struct Kernel {
                     mma_commit(&c->o_step[s]);
                     if (i & 1) {
                         mma_commit(&c->kv_empty[v_stage]);
-                        if (!pair) mma_commit(&c->kv_empty[v_stage]);
                         if (i + 1 == n) mma_commit(&c->o_full[s]);
                     }
                 }
                 __syncwarp();
-                if (i & 1) advance(v_stage, v_phase, step);
+                if (i & 1) {
+                    next_v();
+                    if (!pair && s == 0 && i < r.blocks) pass_v();
+                }
                 if (pair) {
                     if (i + 2 < n) scores(i + 2);
                 } else if ((i & 1) && i + 1 < n) {
                     // K of a stream's next block only after V of this one is free: the two streams would otherwise hold
-                    // four tiles of the ring, and there would be little room to load ahead
+                    // four tiles, and there would be little room to load ahead
                     scores(i + 1);
                     scores(i + 2);
                 }
             }
-            int ahead = 2 * r.blocks % (2 * L::kStages);
-            if (ahead >= L::kStages) ahead -= L::kStages, kv_phase ^= 1;
-            advance(kv_stage, kv_phase, ahead);
+            if (before && r.blocks % 2) {  // the last block, which only stream 0 has
+                pass_k();
+                pass_v();
+            }
         }
         // What the last instructions arrive on is this CTA's memory, and they use tensor memory: both stay until they
         // are done.
@@ -848,7 +869,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&c->q_full[i], 1);
-            mbar_init(&c->q_empty[i], 2);
+            mbar_init(&c->q_empty[i], 2 - i);  // the first tile of queries goes through both streams
             for (int j = 0; j < 4; ++j) mbar_init(&c->turn[i][j], 1);
             for (int j = 0; j < 2; ++j) {
                 mbar_init(&c->s_full[i][j], 1);
@@ -1045,8 +1066,7 @@ int launch(KernelArgs &g, int dtype, int device, bool join, cudaStream_t st) {
 
 }  // namespace
 
-size_t paged_attention_workspace(int64_t rows, int q_heads, int kv_heads, int dim, int seqs, int device) {
-    (void)rows, (void)q_heads, (void)kv_heads, (void)seqs;
+size_t paged_attention_workspace(int dim, int device) {
     const int sms = sm_count(device);
     return shared_bytes(sms) + 2 * static_cast<size_t>(sms) * slot_bytes(dim <= 64 ? 64 : 128);
 }

@@ -17,6 +17,7 @@ a captured CUDA graph follows what they hold when it is replayed.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
@@ -27,6 +28,7 @@ from .. import _native
 __all__ = ["rotary_frequencies", "rotary", "paged_append", "paged_attention"]
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_CACHE_TYPES = (torch.bfloat16, torch.float16)
 _INDEX = {torch.int32: 0, torch.int64: 1}
 
 
@@ -73,16 +75,22 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
     return freq.to(device) if device is not None else freq
 
 
+# A call of a few tokens is over on the GPU in microseconds, so the checks below read each tensor's shape, strides and
+# device once, and compare plain integers.
+
+_current_stream = torch._C._cuda_getCurrentRawStream  # of a device's number
+
+
 def _check(err: int, what: str) -> None:
     if err != 0:
         raise RuntimeError(f"mpcomm {what} failed with CUDA error {err}")
 
 
-def _stream(stream: Optional[torch.cuda.Stream], device: torch.device) -> int:
+def _stream(stream: Optional[torch.cuda.Stream], device: int) -> int:
     if stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    if stream.device != device:
-        raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
+        return _current_stream(device)
+    if stream.device.index != device:
+        raise ValueError(f"stream is on {stream.device}, the tensors on cuda:{device}")
     return stream.cuda_stream
 
 
@@ -94,33 +102,37 @@ def _empty(like: torch.Tensor, shape, dtype, stream: Optional[torch.cuda.Stream]
         return torch.empty(shape, dtype=dtype, device=like.device)
 
 
-def _on_gpu(what: str, device: torch.device) -> None:
-    if device.type != "cuda":
-        raise ValueError(f"mpcomm {what} runs on CUDA tensors, not on {device}")
+def _on_gpu(what: str, device: int) -> None:
+    if device < 0:
+        raise ValueError(f"mpcomm {what} runs on CUDA tensors")
 
 
-def _index(t: torch.Tensor, what: str, device: torch.device) -> int:
+def _index(t: torch.Tensor, what: str, device: int) -> int:
     kind = _INDEX.get(t.dtype)
-    if kind is None or t.device != device:
-        raise ValueError(f"{what} must be an int32 or int64 tensor on {device}")
+    if kind is None or t.get_device() != device:
+        raise ValueError(f"{what} must be an int32 or int64 tensor on the other tensors' device")
     return kind
 
 
-def _frequencies(inv_freq: torch.Tensor, dim: int, device: torch.device) -> None:
-    if inv_freq.dtype not in (torch.float64, torch.float32) or inv_freq.dim() != 1 or inv_freq.device != device \
+def _frequencies(inv_freq: torch.Tensor, dim: int, device: int) -> int:
+    """The number of pairs."""
+    if inv_freq.dtype not in (torch.float64, torch.float32) or inv_freq.dim() != 1 or inv_freq.get_device() != device \
             or not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq must be a contiguous float64 or float32 vector on {device}")
-    if not 0 < 2 * inv_freq.numel() <= dim:
-        raise ValueError(f"inv_freq has {inv_freq.numel()} pairs, a head of {dim} has room for 1 to {dim // 2}")
+        raise ValueError("inv_freq must be a contiguous float64 or float32 vector on the other tensors' device")
+    pairs = inv_freq.shape[0]
+    if not 0 < 2 * pairs <= dim:
+        raise ValueError(f"inv_freq has {pairs} pairs, a head of {dim} has room for 1 to {dim // 2}")
+    return pairs
 
 
-def _no_gradient(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"mpcomm {what} has no gradient: call it under torch.no_grad()")
+def _no_gradient(what: str) -> None:
+    raise RuntimeError(f"mpcomm {what} has no gradient: call it under torch.no_grad()")
 
 
 def _own_memory(t: torch.Tensor, what: str) -> None:
     """Refuses a destination two of whose elements share a place."""
+    if t.is_contiguous():
+        return
     reach = 0
     for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n > 1):
         if stride <= reach:
@@ -129,16 +141,20 @@ def _own_memory(t: torch.Tensor, what: str) -> None:
 
 
 def _turn(x, positions, inv_freq, interleaved, magnitude, sign, out, stream):
-    four = x.dim() == 4
-    heads, dim = x.shape[-2:]
-    batch, tokens = (x.shape[0], x.shape[1]) if four else (1, x.shape[0])
-    xs, os = x.stride(), out.stride()
-    ps = positions.stride()
-    group = (x.data_ptr(), out.data_ptr(), xs[0] if four else 0, *xs[-3:], os[0] if four else 0, *os[-3:], heads, 1, -1)
-    _check(_native.kv_rows([group], dim, inv_freq.numel(), interleaved, batch * tokens, tokens, inv_freq.data_ptr(),
-                           inv_freq.dtype == torch.float64, magnitude, sign, positions.data_ptr(),
-                           _INDEX[positions.dtype], ps[0] if positions.dim() == 2 else 0, ps[-1], None,
-                           _TYPES[x.dtype], x.device.index, _stream(stream, x.device), 0), "rotary")
+    shape, xs, os, ps, device = x.shape, x.stride(), out.stride(), positions.stride(), x.get_device()
+    if len(shape) == 4:
+        batch, tokens, heads, dim = shape
+        group = (x.data_ptr(), out.data_ptr(), *xs, *os, heads, 1, -1)
+    else:
+        tokens, heads, dim = shape
+        batch = 1
+        group = (x.data_ptr(), out.data_ptr(), 0, *xs, 0, *os, heads, 1, -1)
+    err = _native.kv_rows((group,), dim, inv_freq.shape[0], interleaved, batch * tokens, tokens, inv_freq.data_ptr(),
+                          inv_freq.dtype is torch.float64, magnitude, sign, positions.data_ptr(),
+                          _INDEX[positions.dtype], ps[0] if len(ps) == 2 else 0, ps[-1], None, _TYPES[x.dtype], device,
+                          _stream(stream, device), 0)
+    if err:
+        _check(err, "rotary")
     return out
 
 
@@ -173,58 +189,72 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     ``out`` and ``stream``. As with any autograd graph that is captured into a CUDA graph, capture the forward and
     the backward pass together, and let no eager graph of the same leaves live meanwhile.
     """
-    if x.dim() not in (3, 4) or x.dtype not in _TYPES:
+    shape, device = x.shape, x.get_device()
+    if len(shape) not in (3, 4) or x.dtype not in _TYPES:
         raise ValueError("x must be a [(batch,) tokens, heads, head_dim] bf16, fp16 or fp32 tensor")
-    device = x.device
     _index(positions, "positions", device)
-    if positions.shape != x.shape[:-2] and not (x.dim() == 4 and positions.shape == x.shape[1:2]):
-        raise ValueError(f"positions {tuple(positions.shape)} do not fit x {tuple(x.shape)}")
-    _frequencies(inv_freq, x.shape[-1], device)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if positions.shape != shape[:-2] and not (len(shape) == 4 and positions.shape == shape[1:2]):
+        raise ValueError(f"positions {tuple(positions.shape)} do not fit x {tuple(shape)}")
+    _frequencies(inv_freq, shape[-1], device)
+    if x.requires_grad and torch.is_grad_enabled():
         if out is not None or stream is not None:
             raise ValueError("rotary has a gradient only without out and stream")
         _on_gpu("rotary", device)
         return _Rotary.apply(x, positions, inv_freq, bool(interleaved), float(magnitude), 1.0)
     if out is None:
         _on_gpu("rotary", device)
-        out = _empty(x, x.shape, x.dtype, stream)
+        out = _empty(x, shape, x.dtype, stream)
     else:
-        if out.shape != x.shape or out.dtype != x.dtype or out.device != device:
+        if out.shape != shape or out.dtype != x.dtype or out.get_device() != device:
             raise ValueError("out must have the shape, type and device of x")
-        _no_gradient("rotary", out)
+        if out.requires_grad and torch.is_grad_enabled():
+            _no_gradient("rotary into out")
         _own_memory(out, "out")
-    _on_gpu("rotary", device)
-    if x.numel() == 0:
-        return out
-    return _turn(x, positions, inv_freq, bool(interleaved), float(magnitude), 1.0, out, stream)
+        _on_gpu("rotary", device)
+    return _turn(x, positions, inv_freq, bool(interleaved), float(magnitude), 1.0, out, stream) if 0 not in shape else out
 
 
 def _batch(pool, page_table, seq_lens, query_starts, device):
-    if pool.dim() != 5 or pool.shape[1] != 2 or pool.dtype not in (torch.bfloat16, torch.float16):
+    """The cache's shape and the batch as the native calls take it."""
+    shape = pool.shape
+    if len(shape) != 5 or shape[1] != 2 or pool.dtype not in _CACHE_TYPES:
         raise ValueError("the cache must be a [pages, 2, kv_heads, page_tokens, head_dim] bf16 or fp16 tensor")
-    kinds = (_index(page_table, "page_table", device), _index(seq_lens, "seq_lens", device),
-             _index(query_starts, "query_starts", device))
-    if page_table.dim() != 2 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError("page_table must be [seqs, width] with unit stride in a row")
+    if 0 in shape[2:]:
+        raise ValueError("the cache has no heads, no tokens in a page or no elements in a head")
+    if page_table.dim() != 2:
+        raise ValueError("page_table must be [seqs, width]")
     seqs, width = page_table.shape
+    row, one = page_table.stride()
+    if one != 1 and width > 1:
+        raise ValueError("page_table must have unit stride in a row")
     if seq_lens.shape != (seqs,) or query_starts.shape != (seqs + 1,):
         raise ValueError(f"a page_table of {seqs} sequences needs seq_lens [{seqs}] and query_starts [{seqs + 1}]")
-    if not seq_lens.is_contiguous() or not query_starts.is_contiguous():
+    if not (seq_lens.is_contiguous() and query_starts.is_contiguous()):
         raise ValueError("seq_lens and query_starts must be contiguous")
-    if 0 in pool.shape[2:]:
-        raise ValueError("the cache has no heads, no tokens in a page or no elements in a head")
-    return (page_table.data_ptr(), kinds[0], page_table.stride(0), width, seq_lens.data_ptr(), kinds[1],
-            query_starts.data_ptr(), kinds[2], seqs, pool.shape[3], pool.shape[0])
+    return shape, (page_table.data_ptr(), _index(page_table, "page_table", device), row, width,
+                   seq_lens.data_ptr(), _index(seq_lens, "seq_lens", device),
+                   query_starts.data_ptr(), _index(query_starts, "query_starts", device), seqs, shape[3], shape[0])
 
 
-def _strides(t: torch.Tensor):
-    """Strides, with those of axes of one element (which are not used) aligned."""
-    return tuple(st if n > 1 else 8 for n, st in zip(t.shape[:-1], t.stride())) + (t.stride(-1),)
+def _rows(t: torch.Tensor, what: str, pool: torch.Tensor, dim: int, device: int):
+    """The shape of a tensor of new tokens."""
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or t.dtype != pool.dtype or t.get_device() != device:
+        raise ValueError(f"{what} must be a [tokens, heads, {dim}] {pool.dtype} tensor on the other tensors' device")
+    return shape
 
 
-def _rows(t: torch.Tensor, what: str, pool: torch.Tensor, device: torch.device) -> None:
-    if t.dim() != 3 or t.dtype != pool.dtype or t.device != device or t.shape[2] != pool.shape[4]:
-        raise ValueError(f"{what} must be a [tokens, heads, {pool.shape[4]}] {pool.dtype} tensor on {device}")
+def _aligned(t: torch.Tensor, shape, what: str):
+    """Strides that wide accesses can take. Those of axes of one element are not used; they are given as 8."""
+    strides = t.stride()
+    if 1 in shape:
+        strides = tuple(st if n > 1 else 8 for n, st in zip(shape[:-1], strides)) + strides[-1:]
+    bits = 0
+    for st in strides[:-1]:
+        bits |= st if st > 0 else 1
+    if strides[-1] != 1 or bits % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{what} must have unit stride in a head, other strides of 16 bytes or multiples, aligned to 16 bytes")
+    return strides
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_table: torch.Tensor,
@@ -245,22 +275,22 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
     and sets bit 2 of the uint32 device word at ``status_ptr``. Slots that two tokens of one call share get one of
     them. bf16 and fp16.
     """
-    device = k.device
-    batch = _batch(pool, page_table, seq_lens, query_starts, device)
-    if pool.device != device and not (pool.device.type == "cpu" and pool.is_pinned()):
-        raise ValueError(f"the cache must lie on {device} or in pinned host memory")
-    _rows(k, "k", pool, device)
-    _rows(v, "v", pool, device)
-    kv_heads, dim = pool.shape[2], pool.shape[4]
-    if k.shape[1] != kv_heads or v.shape != k.shape:
+    device = k.get_device()
+    cache, batch = _batch(pool, page_table, seq_lens, query_starts, device)
+    kv_heads, dim = cache[2], cache[4]
+    if pool.get_device() != device and not (pool.device.type == "cpu" and pool.is_pinned()):
+        raise ValueError("the cache must lie on the other tensors' device or in pinned host memory")
+    shape = _rows(k, "k", pool, dim, device)
+    if shape[1] != kv_heads or _rows(v, "v", pool, dim, device) != shape:
         raise ValueError(f"k and v must have {kv_heads} heads and the same tokens")
-    _no_gradient("paged_append", k, v, q, pool, q_out)
+    if (k.requires_grad or v.requires_grad or pool.requires_grad or (q is not None and q.requires_grad)
+            or (q_out is not None and q_out.requires_grad)) and torch.is_grad_enabled():
+        _no_gradient("paged_append")
     _own_memory(pool, "the cache")
-    rows = k.shape[0]
+    rows = shape[0]
     pairs = freq = wide = 0
     if inv_freq is not None:
-        _frequencies(inv_freq, dim, device)
-        pairs, freq, wide = inv_freq.numel(), inv_freq.data_ptr(), inv_freq.dtype == torch.float64
+        pairs, freq, wide = _frequencies(inv_freq, dim, device), inv_freq.data_ptr(), inv_freq.dtype is torch.float64
     elif q is not None or positions is not None:
         raise ValueError("q and positions need inv_freq")
     pos = pos64 = pos_stride = 0
@@ -269,31 +299,30 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
         if positions.shape != (rows,):
             raise ValueError(f"positions must be [{rows}]")
         pos, pos_stride = positions.data_ptr(), positions.stride(0)
-    ps, size = pool.stride(), pool.element_size()
-    slot = (ps[0], ps[3], ps[2], ps[4], kv_heads)
-    at = pool.data_ptr()
-    groups = [(k.data_ptr(), at, 0, *k.stride(), *slot, pairs > 0, 0),
-              (v.data_ptr(), at + ps[1] * size, 0, *v.stride(), *slot, 0, 1)]
+    page, plane, head, token, element = pool.stride()
+    at, turn = pool.data_ptr(), pairs > 0
+    groups = ((k.data_ptr(), at, 0, *k.stride(), page, token, head, element, kv_heads, turn, 0),
+              (v.data_ptr(), at + plane * 2, 0, *v.stride(), page, token, head, element, kv_heads, 0, 1))
     if q is not None:
-        _rows(q, "q", pool, device)
-        if q.shape[0] != rows:
+        q_shape = _rows(q, "q", pool, dim, device)
+        if q_shape[0] != rows:
             raise ValueError("q must have the tokens of k")
         if q_out is None:
             _on_gpu("paged_append", device)
-            q_out = _empty(q, q.shape, q.dtype, stream)
+            q_out = _empty(q, q_shape, q.dtype, stream)
         else:
-            _rows(q_out, "q_out", pool, device)
-            if q_out.shape != q.shape:
+            if _rows(q_out, "q_out", pool, dim, device) != q_shape:
                 raise ValueError("q_out must have the shape of q")
             _own_memory(q_out, "q_out")
-        groups.append((q.data_ptr(), q_out.data_ptr(), 0, *q.stride(), 0, *q_out.stride(), q.shape[1], 1, -1))
+        groups += ((q.data_ptr(), q_out.data_ptr(), 0, *q.stride(), 0, *q_out.stride(), q_shape[1], 1, -1),)
     elif q_out is not None:
         raise ValueError("q_out needs q")
     _on_gpu("paged_append", device)
     if rows and batch[8]:
-        _check(_native.kv_rows(groups, dim, pairs, bool(interleaved), rows, rows, freq, wide, float(magnitude), 1.0,
-                               pos, pos64, 0, pos_stride, batch, _TYPES[pool.dtype], device.index,
-                               _stream(stream, device), status_ptr), "paged_append")
+        err = _native.kv_rows(groups, dim, pairs, bool(interleaved), rows, rows, freq, wide, float(magnitude), 1.0, pos,
+                              pos64, 0, pos_stride, batch, _TYPES[pool.dtype], device, _stream(stream, device), status_ptr)
+        if err:
+            _check(err, "paged_append")
     return pool if q is None else (pool, q_out)
 
 
@@ -318,46 +347,48 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     bf16 and fp16, ``head_dim`` a multiple of 8 up to 128, ``page_tokens`` a multiple of 8, all strides of ``q``,
     ``out`` and ``pool`` multiples of 16 bytes but the last, which is one element. The cache is in device memory.
     """
-    device = q.device
-    batch = _batch(pool, page_table, seq_lens, query_starts, device)
-    if pool.device != device:
-        raise ValueError(f"the cache must lie on {device}")
-    _rows(q, "q", pool, device)
-    _no_gradient("paged_attention", q, pool, out)
-    kv_heads, page_tokens, dim = pool.shape[2:]
-    rows, q_heads = q.shape[0], q.shape[1]
+    device = q.get_device()
+    cache, batch = _batch(pool, page_table, seq_lens, query_starts, device)
+    _, _, kv_heads, page_tokens, dim = cache
+    if pool.get_device() != device:
+        raise ValueError("the cache must lie on the other tensors' device")
+    shape = _rows(q, "q", pool, dim, device)
+    rows, q_heads, _ = shape
+    if (q.requires_grad or pool.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
+        _no_gradient("paged_attention")
     if q_heads == 0 or q_heads % kv_heads:
         raise ValueError(f"{q_heads} query heads cannot share {kv_heads} key heads")
     if dim % 8 or dim > 128 or page_tokens % 8:
         raise ValueError("head_dim must be a multiple of 8 up to 128, page_tokens a multiple of 8")
     if window < 0 or (window and not causal):
         raise ValueError("window must be positive, and needs causal")
-    ps, qs = _strides(pool), _strides(q)
-    if ps[4] != 1 or (ps[0] | ps[1] | ps[2] | ps[3]) % 8 or pool.data_ptr() % 16 or min(ps) < 1:
-        raise ValueError("the cache must have unit stride in a head and 16-byte aligned strides otherwise")
-    if qs[2] != 1 or (qs[0] | qs[1]) % 8 or q.data_ptr() % 16 or min(qs) < 1:
-        raise ValueError("q must have unit stride in a head and 16-byte aligned strides otherwise")
+    page, plane, head, token, _ = _aligned(pool, cache, "the cache")
+    q_token, q_head, _ = _aligned(q, shape, "q")
     fresh = out is None
     if fresh:
         _on_gpu("paged_attention", device)
-        out = _empty(q, q.shape, q.dtype, stream)
+        out = _empty(q, shape, q.dtype, stream)
     else:
-        _rows(out, "out", pool, device)
-        if out.shape != q.shape:
+        if _rows(out, "out", pool, dim, device) != shape:
             raise ValueError("out must have the shape of q")
         _own_memory(out, "out")
-    os = _strides(out)
-    if os[2] != 1 or (os[0] | os[1]) % 8 or out.data_ptr() % 16:
-        raise ValueError("out must have unit stride in a head and 16-byte aligned strides otherwise")
+    o_token, o_head, _ = _aligned(out, shape, "out")
     _on_gpu("paged_attention", device)
     lse = _empty(q, (rows, q_heads), torch.float32, stream) if return_lse else None
     if rows:
-        need = _native.paged_attention_workspace(rows, q_heads, kv_heads, dim, batch[8], device.index)
-        space = _empty(q, (need,), torch.uint8, stream) if need else None
-        _check(_native.paged_attention(
-            q.data_ptr(), qs[0], qs[1], out.data_ptr(), os[0], os[1], lse.data_ptr() if return_lse else 0,
-            pool.data_ptr(), ps[0], ps[1], ps[2], ps[3], rows, q_heads, kv_heads, dim,
-            dim ** -0.5 if scale is None else float(scale), bool(causal), int(window), fresh, batch,
-            space.data_ptr() if need else 0, need, _TYPES[pool.dtype], device.index, _stream(stream, device),
-            status_ptr), "paged_attention")
+        need = _workspace(dim > 64, device)
+        space = _empty(q, need, torch.uint8, stream)
+        err = _native.paged_attention(
+            q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, lse.data_ptr() if return_lse else 0,
+            pool.data_ptr(), page, plane, head, token, rows, q_heads, kv_heads, dim,
+            dim ** -0.5 if scale is None else float(scale), bool(causal), window, fresh, batch, space.data_ptr(), need,
+            _TYPES[pool.dtype], device, _stream(stream, device), status_ptr)
+        if err:
+            _check(err, "paged_attention")
     return (out, lse) if return_lse else out
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace(wide: bool, device: int) -> int:
+    """Bytes that a call needs on a device, whatever its sizes but for heads of over 64 elements."""
+    return _native.paged_attention_workspace(128 if wide else 64, device)

@@ -918,8 +918,7 @@ PYBIND11_MODULE(_mpcomm, m) {
         py::arg("batch"), py::arg("dtype"), py::arg("device"), py::arg("stream"), py::arg("status") = 0,
         "Rotates and copies rows of heads; each group is (src, dst, four source strides, four destination strides, "
         "heads, rotate, cache plane or -1), batch the paged batch's description or None.");
-    m.def("paged_attention_workspace", &kern::paged_attention_workspace, py::arg("rows"), py::arg("q_heads"),
-          py::arg("kv_heads"), py::arg("dim"), py::arg("seqs"), py::arg("device"),
+    m.def("paged_attention_workspace", &kern::paged_attention_workspace, py::arg("dim"), py::arg("device"),
           "Bytes of workspace that paged_attention needs (any contents, 16-byte aligned).");
     m.def(
         "paged_attention",

@@ -531,3 +531,20 @@ def test_parts_of_a_context_join_by_their_log_sum_exp():
     # each part is rounded to the type once more, and its own weights: twice the tolerance of one
     size = torch.maximum(head[0].abs(), tail[0].abs()).double()
     _near(joined, want, 2 * tol + size * 2.0 ** -8)
+
+
+@pytest.mark.parametrize("news,lens", [
+    ([512] * 8, [512] * 8),  # many short runs of two full streams
+    ([1, 300] * 10, [40, 300] * 10),  # single tokens and chunks in turn
+    ([1] * 64, [130 + 61 * i for i in range(64)]),  # more sequences than a warp, odd numbers of blocks
+    ([1] * 70 + [200], list(range(1, 141, 2)) + [900]),
+])
+def test_attention_over_many_runs_back_to_back(news, lens):
+    """Runs of one and of two streams in one CTA, call after call: every call the same, and right."""
+    args, how = _attention_case(news, lens, q_heads=32, kv_heads=8, spoil=True, seed=30)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    _check_attention(args, how, news)
+    first = ops.paged_attention(*args)
+    for _ in range(200):
+        again = ops.paged_attention(*args, status_ptr=status.data_ptr())
+    assert torch.equal(again, first) and status.item() == 0
