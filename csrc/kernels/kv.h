@@ -29,6 +29,20 @@ struct IndexPtr {
     }
 };
 
+// Division of 31-bit values by a constant: a multiplication.
+struct FastDiv {
+    uint32_t times = 0, shift = 0;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d) {
+        // 2^(31 + ceil(log2 d)) / d, rounded up, is at most 2^32 - 1 and exact for 31-bit dividends
+        while ((1ull << shift) < d) ++shift;
+        times = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
+    }
+    MPCOMM_HD int div(int n) const {
+        return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * times) >> (31 + shift));
+    }
+};
+
 // A ragged batch over a paged cache. Rows starts[b] .. starts[b + 1] are the
 // newest tokens of sequence b, lens[b] counts all its tokens. Token p lies
 // in slot p % page_tokens of page table[b * table_stride + p / page_tokens].
@@ -82,7 +96,7 @@ struct KvRowsArgs {
     int dim = 0;
     int pairs = 0;  // rotated pairs of a head
     int interleaved = 0;
-    int64_t rows = 0, tokens = 1;
+    int64_t rows = 0, tokens = 1;  // below 2^31
     const void *inv_freq = nullptr;  // radians a position, one for each pair
     int freq_f64 = 0;
     float magnitude = 1.f, sign = 1.f;

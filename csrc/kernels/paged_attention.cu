@@ -125,20 +125,6 @@ struct PoolView {
     int group_bytes, half_bytes;  // in shared memory: distance of 8-row groups, of halves
 };
 
-// Division of 31-bit values by a constant: a multiplication.
-struct FastDiv {
-    uint32_t times = 0, shift = 0;
-    FastDiv() = default;
-    explicit FastDiv(uint32_t d) {
-        // 2^(31 + ceil(log2 d)) / d, rounded up, is at most 2^32 - 1 and exact for 31-bit dividends
-        while ((1ull << shift) < d) ++shift;
-        times = static_cast<uint32_t>(((1ull << (31 + shift)) + d - 1) / d);
-    }
-    __device__ __forceinline__ int div(int n) const {
-        return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * times) >> (31 + shift));
-    }
-};
-
 struct KernelArgs {
     PagedAttentionArgs a;
     PlanShape shape;

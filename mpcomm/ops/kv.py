@@ -120,8 +120,8 @@ def _frequencies(inv_freq: torch.Tensor, dim: int, device: int) -> int:
             or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float64 or float32 vector on the other tensors' device")
     pairs = inv_freq.shape[0]
-    if not 0 < 2 * pairs <= dim:
-        raise ValueError(f"inv_freq has {pairs} pairs, a head of {dim} has room for 1 to {dim // 2}")
+    if not 0 < 2 * pairs <= min(dim, 8192):
+        raise ValueError(f"inv_freq has {pairs} pairs, a head of {dim} has room for 1 to {min(dim, 8192) // 2}")
     return pairs
 
 
@@ -171,7 +171,13 @@ class _Rotary(torch.autograd.Function):
         positions, inv_freq = ctx.saved_tensors
         interleaved, magnitude, sign = ctx.how
         # the rotation is linear and its transpose is the rotation back, so a gradient of the gradient is one more
-        return _Rotary.apply(grad, positions, inv_freq, interleaved, magnitude, -sign), None, None, None, None, None
+        if grad.requires_grad and torch.is_grad_enabled():
+            back = _Rotary.apply(grad, positions, inv_freq, interleaved, magnitude, -sign)
+        else:
+            back = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device)
+            if grad.numel():
+                _turn(grad, positions, inv_freq, interleaved, magnitude, -sign, back, None)
+        return back, None, None, None, None, None
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,

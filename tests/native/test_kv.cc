@@ -59,6 +59,14 @@ static void test_div() {
     for (int64_t a : v)
         for (int64_t b : v)
             if (b) CHECK(plan_div(a, b) == a / b);
+    std::mt19937 rng(3);
+    for (uint32_t d = 1; d < 70000; d += d < 300 ? 1 : 1 + rng() % 97) {
+        const FastDiv f(d);
+        for (uint32_t n : {0u, 1u, d - 1, d, d + 1, 0x7fffffffu, 0x7fffffffu / d * d, 0x7fffffffu / d * d - 1, static_cast<uint32_t>(rng() >> 1)})
+            CHECK(n > 0x7fffffffu || f.div(static_cast<int>(n)) == static_cast<int>(n / d));
+    }
+    for (uint32_t d : {0x40000000u, 0x7fffffffu, 0x10000001u})
+        CHECK(FastDiv(d).div(0x7fffffff) == static_cast<int>(0x7fffffffu / d) && FastDiv(d).div(static_cast<int>(d) - 1) == 0);
 }
 
 static void check_plan(const PlanShape &s, const std::vector<int64_t> &starts, const std::vector<int64_t> &lens, int ctas) {

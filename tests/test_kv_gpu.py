@@ -30,7 +30,8 @@ def _near(got, want, tolerance, what=""):
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("tokens,heads,dim,part", [(1, 1, 2, 2), (1, 40, 128, 128), (37, 3, 96, 48), (130, 5, 80, 80),
-                                                   (5, 7, 10, 6), (3, 2, 256, 256), (700, 33, 64, 32)])
+                                                   (5, 7, 10, 6), (3, 2, 256, 256), (700, 33, 64, 32),
+                                                   (2, 3, 1030, 514), (9000, 5, 128, 128)])
 def test_rotary_matches_the_formula(dtype, interleaved, tokens, heads, dim, part):
     x = _randn(tokens, heads, dim, dtype=dtype, seed=tokens)
     freq = ops.rotary_frequencies(part, 500000.0, "linear", 4.0, device="cuda")
@@ -174,6 +175,7 @@ def _expect_append(pool, k, v, table, lens, starts, rotate=None):
     (BF16, 3, 80, 24, [50], [90]),
     (FP16, 1, 10, 5, [7, 3], [7, 6]),
     (BF16, 4, 128, 1, [3, 2], [3, 9]),
+    (BF16, 1, 16, 8, [b % 3 for b in range(1100)], [b % 3 + b % 40 for b in range(1100)]),
 ])
 def test_append_stores_every_token_in_its_slot(token_major, dtype, heads, dim, page_tokens, news, lens):
     table, lens, starts, pages = ref.batch(news, lens, page_tokens, device="cuda")
