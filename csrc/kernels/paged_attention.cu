@@ -55,7 +55,6 @@ constexpr int kRunSlots = 4;
 constexpr int kFewTiles = 4;  // of a sequence, that one lane counts
 constexpr int kMaskSlots = 16;  // blocks whose masks are kept: more than are ever in flight
 constexpr float kRescale = 8.f;
-constexpr int kFmaPairs = 2;  // of 16 pairs of scores, whose exponentials are taken on the FMA pipes
 
 __device__ uint32_t g_attention_status;
 
@@ -611,8 +610,9 @@ struct Kernel {
         return max_nan(max_nan(t[0], t[1]), t[2], t[3]);
     }
 
-    // Scores to weights: x[j] = 2^(x[j] * times + less), and the weights in 16 bits to tensor memory. Some
-    // exponentials go to the FMA pipes: the special function unit alone takes 512 cycles for a warp's rows.
+    // Scores to weights: x[j] = 2^(x[j] * times + less), and the weights in 16 bits to tensor memory. All
+    // exponentials go to the special function unit (512 cycles for a warp's half block). Two to six of 16 by
+    // polynomials on the FMA pipes instead were slower: a step waits for latencies, not for that unit.
     static __device__ __forceinline__ void weigh(uint32_t (&x)[32], float times, float less, uint32_t to) {
         const Pair times2 = make_pair(times, times), less2 = make_pair(less, less);
         uint32_t p[16];
@@ -620,12 +620,8 @@ struct Kernel {
         for (int e = 0; e < 16; ++e) {
             float u, v;
             split(fma2(make_pair(x[2 * e], x[2 * e + 1]), times2, less2), u, v);
-            if (e * kFmaPairs % 16 < kFmaPairs) {
-                split(exp2_fma(u, v), u, v);
-            } else {
-                u = exp2_approx(u);
-                v = exp2_approx(v);
-            }
+            u = exp2_approx(u);
+            v = exp2_approx(v);
             p[e] = pack(u, v);
             x[2 * e] = __float_as_uint(u);
             x[2 * e + 1] = __float_as_uint(v);
@@ -668,79 +664,69 @@ struct Kernel {
             }
             // keys that every row of the warp sees: blocks inside need no mask
             const int all_lo = __reduce_max_sync(~0u, lo), all_hi = __reduce_min_sync(~0u, hi);
-            bool huge = false;  // some row's m is too large for one rounding (below)
-            float m = -INFINITY, ref = 0.f, less = 0.f, sum = 0.f;  // m = ref * scale, less = -m
+            // m, the reference, is ref * scale, rounded; a weight is 2^(x * times + less).
+            float m = -INFINITY, ref = 0.f, times = scale, less = 0.f, sum = 0.f;
+            // A half block from its scores to its weights. Masked ones are rare and have code of their own, away from
+            // the loop's: the instructions that a step goes past cost it as much as some that it executes.
+            auto step = [&](int i, uint32_t ts, uint32_t (&x)[2][32]) {
+                const float top = largest(x), next = top * scale;
+                const bool move = !(next <= m + kRescale);  // NaN moves it too
+                if (__builtin_expect(__any_sync(~0u, move && live), 0)) {
+                    const float was = m;
+                    if (move) {
+                        m = next;
+                        ref = top;
+                        // What m was rounded by is the same for the whole row and cancels. Where it could be many
+                        // powers of two (the lowest value of a type as a score) the scores are taken times a power of
+                        // two instead, which rounds nothing: equal scores have equal weights, and others none.
+                        const bool far = fabsf(m) > 0x1p26f;
+                        times = far ? __uint_as_float(__float_as_uint(scale) & 0x7f800000u) : scale;
+                        // the weights of a row with a NaN or an infinite score are NaN; nothing seen yet: zero
+                        less = m == -INFINITY ? 0.f : m == INFINITY ? NAN : far ? -ref * times : -m;
+                    }
+                    if (i > 0) {
+                        const float keep = move ? exp2_approx(was - m) : 1.f;
+                        sum *= keep;
+                        // The output so far is complete when the last half block's weights have been used (the one
+                        // before has: its buffer holds these scores). n_s counts this half block already.
+                        wait(&c->o_step[s], n_s & 1);
+                        tmem_fence_after();
+#pragma unroll 1
+                        for (int j = 0; j < a.dim; j += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(to + j, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st16(to + j, o);
+                        }
+                    }
+                }
+                if (pair) wait(&c->turn[s][warp], (n_turn++ & 1) ^ (s == 0));
+                weigh(x[0], times, less, ts);
+                weigh(x[1], times, less, ts + 16);
+                if (pair && lane == 0) mbar_arrive(&c->turn[s ^ 1][warp]);
+                hand_over(&c->p_full[s][i & 1]);
+                // the sum is taken while the tensor core has the weights
+                Pair add[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t *y = x[j / 2] + j % 2 * 16;
+                    add[j] = make_pair(y[0], y[1]);
+#pragma unroll
+                    for (int e = 2; e < 16; e += 2) add[j] = add2(add[j], make_pair(y[e], y[e + 1]));
+                }
+                float s0, s1;
+                split(add2(add2(add[0], add[1]), add2(add[2], add[3])), s0, s1);
+                sum += s0 + s1;
+            };
             for (int i = 0; i < 2 * steps; ++i) {
                 const int half = i & 1, block = pair ? i / 2 : i / 2 * 2 + s;
                 const int key0 = r.key0 + block * kBlockKeys + half * kHalfKeys;
                 const uint32_t ts = tmem + s_at(s, half) + lanes;
                 wait(&c->s_full[s][half], n_s++ >> 1 & 1);
                 tmem_fence_after();
-                if (work) {
-                    uint32_t x[2][32];
-                    tmem_ld32(ts, x[0]);
-                    tmem_ld32(ts + 32, x[1]);
-                    const uint32_t boxes = c->mask[(n_block + block) % kMaskSlots];
-                    tmem_wait_ld();
-                    if (__builtin_expect(all_hi < key0 + kHalfKeys || all_lo > key0 || boxes != ~0u, 0))
-                        mask_scores(x, lo - key0, hi - key0, half * kHalfKeys, boxes);
-                    const float top = largest(x);
-                    // m, a reference in units of log2
-                    const float next = top * scale;
-                    const bool move = !(next <= m + kRescale);  // NaN moves it too
-                    if (__builtin_expect(__any_sync(~0u, move && live), 0)) {
-                        const float was = m;
-                        if (move) m = next, ref = top;
-                        // the weights of a row with a NaN or an infinite score are NaN; nothing seen yet: zero
-                        less = m == -INFINITY ? 0.f : m == INFINITY ? NAN : -m;
-                        // x * scale - m is off by what m was rounded by, the same for the whole row, so it cancels;
-                        // where it could pass 1 (the lowest value of a type as a score) the reference comes off first.
-                        huge = __any_sync(~0u, live && fabsf(m) > 0x1p24f && m != -INFINITY);
-                        if (i > 0) {
-                            const float keep = move ? exp2_approx(was - m) : 1.f;
-                            sum *= keep;
-                            // The output so far is complete when the last half block's weights have been used (the
-                            // one before has: its buffer holds these scores). n_s counts this half block already.
-                            wait(&c->o_step[s], n_s & 1);
-                            tmem_fence_after();
-#pragma unroll 1
-                            for (int j = 0; j < a.dim; j += 16) {
-                                uint32_t o[16];
-                                tmem_ld16(to + j, o);
-                                tmem_wait_ld();
-#pragma unroll
-                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                                tmem_st16(to + j, o);
-                            }
-                        }
-                    }
-                    float times = scale, minus = less;
-                    if (__builtin_expect(huge, 0)) {
-                        const float off = m == -INFINITY ? 0.f : ref;
-#pragma unroll
-                        for (int j = 0; j < kHalfKeys; ++j)
-                            x[j / 32][j % 32] = __float_as_uint((__uint_as_float(x[j / 32][j % 32]) - off) * scale);
-                        minus = less * 0.f;
-                        times = 1.f;
-                    }
-                    if (pair) wait(&c->turn[s][warp], (n_turn++ & 1) ^ (s == 0));
-                    weigh(x[0], times, minus, ts);
-                    weigh(x[1], times, minus, ts + 16);
-                    if (pair && lane == 0) mbar_arrive(&c->turn[s ^ 1][warp]);
-                    hand_over(&c->p_full[s][half]);
-                    // the sum is taken while the tensor core has the weights
-                    Pair add[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t *y = x[j / 2] + j % 2 * 16;
-                        add[j] = make_pair(y[0], y[1]);
-#pragma unroll
-                        for (int e = 2; e < 16; e += 2) add[j] = add2(add[j], make_pair(y[e], y[e + 1]));
-                    }
-                    float s0, s1;
-                    split(add2(add2(add[0], add[1]), add2(add[2], add[3])), s0, s1);
-                    sum += s0 + s1;
-                } else {
+                if (!work) {
                     if (pair) wait(&c->turn[s][warp], (n_turn++ & 1) ^ (s == 0));
                     tmem_fence_before();
                     __syncwarp();
@@ -748,6 +734,18 @@ struct Kernel {
                         if (pair) mbar_arrive(&c->turn[s ^ 1][warp]);
                         mbar_arrive(&c->p_full[s][half]);
                     }
+                    continue;
+                }
+                uint32_t x[2][32];
+                tmem_ld32(ts, x[0]);
+                tmem_ld32(ts + 32, x[1]);
+                const uint32_t boxes = c->mask[(n_block + block) % kMaskSlots];
+                tmem_wait_ld();
+                if (__builtin_expect(all_hi >= key0 + kHalfKeys && all_lo <= key0 && boxes == ~0u, 1)) {
+                    step(i, ts, x);
+                } else {
+                    mask_scores(x, lo - key0, hi - key0, half * kHalfKeys, boxes);
+                    step(i, ts, x);
                 }
             }
             n_block += r.blocks;

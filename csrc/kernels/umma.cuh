@@ -214,24 +214,5 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     return y;
 }
 
-// 2^x of two values on the FMA pipes, for x <= 127; below -126 it is 2^-126.
-// x = n + f with n whole and |f| <= 1/2 (adding 1.5 * 2^23 leaves n in the low
-// bits), 2^f by a polynomial of degree 5 fitted for the least relative error
-// (2.3e-7 in 32-bit arithmetic), and n goes into the exponent.
-__device__ __forceinline__ Pair exp2_fma(float lo, float hi) {
-    const Pair x = make_pair(max_nan(lo, -126.f), max_nan(hi, -126.f));
-    const Pair t = add2(x, make_pair(12582912.f, 12582912.f));
-    const Pair n = add2(t, make_pair(-12582912.f, -12582912.f));
-    const Pair f = fma2(n, make_pair(-1.f, -1.f), x);
-    constexpr float c[6] = {0x1.000002p+0f, 0x1.62e428p-1f, 0x1.ebf918p-3f, 0x1.c6b6e4p-5f, 0x1.3d0c52p-7f, 0x1.5c08e4p-10f};
-    Pair p = make_pair(c[5], c[5]);
-#pragma unroll
-    for (int i = 4; i >= 0; --i) p = fma2(p, f, make_pair(c[i], c[i]));
-    float p0, p1, t0, t1;
-    split(p, p0, p1);
-    split(t, t0, t1);
-    return make_pair(__float_as_uint(p0) + (__float_as_uint(t0) << 23), __float_as_uint(p1) + (__float_as_uint(t1) << 23));
-}
-
 }  // namespace kern
 }  // namespace mpcomm

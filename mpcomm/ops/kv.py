@@ -160,24 +160,25 @@ def _turn(x, positions, inv_freq, interleaved, magnitude, sign, out, stream):
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, positions, inv_freq, interleaved, magnitude, sign):
+    def forward(ctx, x, positions, inv_freq, how):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.how = (interleaved, magnitude, sign)
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        return _turn(x, positions, inv_freq, interleaved, magnitude, sign, out, None) if x.numel() else out
+        ctx.how = how
+        shape = x.shape
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        return out if 0 in shape else _turn(x, positions, inv_freq, *how, out, None)
 
     @staticmethod
     def backward(ctx, grad):
+        # the rotation is linear and its transpose is the rotation back, so a gradient of the gradient is one more
         positions, inv_freq = ctx.saved_tensors
         interleaved, magnitude, sign = ctx.how
-        # the rotation is linear and its transpose is the rotation back, so a gradient of the gradient is one more
         if grad.requires_grad and torch.is_grad_enabled():
-            back = _Rotary.apply(grad, positions, inv_freq, interleaved, magnitude, -sign)
-        else:
-            back = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device)
-            if grad.numel():
-                _turn(grad, positions, inv_freq, interleaved, magnitude, -sign, back, None)
-        return back, None, None, None, None, None
+            return _Rotary.apply(grad, positions, inv_freq, (interleaved, magnitude, -sign)), None, None, None
+        shape = grad.shape
+        out = torch.empty(shape, dtype=grad.dtype, device=grad.device)
+        if 0 not in shape:
+            _turn(grad, positions, inv_freq, interleaved, magnitude, -sign, out, None)
+        return out, None, None, None
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, interleaved: bool = False,
@@ -206,7 +207,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
         if out is not None or stream is not None:
             raise ValueError("rotary has a gradient only without out and stream")
         _on_gpu("rotary", device)
-        return _Rotary.apply(x, positions, inv_freq, bool(interleaved), float(magnitude), 1.0)
+        return _Rotary.apply(x, positions, inv_freq, (bool(interleaved), float(magnitude), 1.0))
     if out is None:
         _on_gpu("rotary", device)
         out = _empty(x, shape, x.dtype, stream)
