@@ -684,7 +684,7 @@ struct Kernel {
                         // the weights of a row with a NaN or an infinite score are NaN; nothing seen yet: zero
                         less = m == -INFINITY ? 0.f : m == INFINITY ? NAN : far ? -ref * times : -m;
                     }
-                    if (i > 0) {
+                    if (__any_sync(~0u, move && live && was != -INFINITY)) {  // a row without weights so far has no output
                         const float keep = move ? exp2_approx(was - m) : 1.f;
                         sum *= keep;
                         // The output so far is complete when the last half block's weights have been used (the one
@@ -692,13 +692,13 @@ struct Kernel {
                         wait(&c->o_step[s], n_s & 1);
                         tmem_fence_after();
 #pragma unroll 1
-                        for (int j = 0; j < a.dim; j += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(to + j, o);
+                        for (int j = 0; j < a.dim; j += 32) {
+                            uint32_t o[32];
+                            tmem_ld32(to + j, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                            tmem_st16(to + j, o);
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+                            tmem_st32(to + j, o);
                         }
                     }
                 }
@@ -782,6 +782,8 @@ struct Kernel {
                 const int slot_row = (pair ? s * kStreamRows : 0) + row;
                 char *slot = static_cast<char *>(a.workspace) + shared_bytes(g.ctas) + (2 * blockIdx.x + r.slot) * slot_bytes(DP);
                 T *out = static_cast<T *>(a.out) + q_row * a.o_st + head * a.o_sh;
+                // rows of whole sectors: half the stores
+                const bool sectors = ((reinterpret_cast<uintptr_t>(a.out) & 31) | (a.o_st | a.o_sh | a.dim) % 16) == 0;
                 if (r.slot < 0) {
                     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
                     k0 *= inv;
@@ -801,17 +803,30 @@ struct Kernel {
                         if (both) f[e] = fmaf(__uint_as_float(o1[e]), k1, f[e]);
                         if (sum == 0.f) f[e] = 0.f;
                     }
-                    if (r.slot < 0) {
+                    if (r.slot >= 0) {
+                        float *o32 = reinterpret_cast<float *>(slot) + slot_row * DP + j;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint32_t p[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) p[k] = __float_as_uint(f[e + k]);
+                            st_sector(o32 + e, p);
+                        }
+                    } else if (sectors) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 16) {
+                            uint32_t p[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) p[k] = pack(f[e + 2 * k], f[e + 2 * k + 1]);
+                            if (j + e < a.dim) st_sector(out + j + e, p);
+                        }
+                    } else {
 #pragma unroll
                         for (int e = 0; e < 32; e += 8)
                             if (j + e < a.dim)
                                 *reinterpret_cast<uint4 *>(out + j + e) =
                                     make_uint4(pack(f[e], f[e + 1]), pack(f[e + 2], f[e + 3]), pack(f[e + 4], f[e + 5]),
                                                pack(f[e + 6], f[e + 7]));
-                    } else {
-                        float *o32 = reinterpret_cast<float *>(slot) + slot_row * DP + j;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4 *>(o32 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
                     }
                 }
                 if (live && r.slot >= 0)
