@@ -550,3 +550,22 @@ def test_attention_over_many_runs_back_to_back(news, lens):
     for _ in range(200):
         again = ops.paged_attention(*args, status_ptr=status.data_ptr())
     assert torch.equal(again, first) and status.item() == 0
+
+
+def test_attention_workspaces_of_any_contents():
+    """Memory that was marked by other calls, and a captured call replayed with others between."""
+    args, how = _attention_case([1] * 3 + [90], [5000, 900, 20, 3000], q_heads=16, kv_heads=4, seed=31)
+    other, _ = _attention_case([1] * 6, [4000] * 6, q_heads=8, kv_heads=1, dim=64, seed=32)
+    want, want_other = ops.paged_attention(*args), ops.paged_attention(*other)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_attention(*args)
+    for n in range(30):
+        junk = torch.randint(0, 256, (48 << 20,), dtype=torch.uint8, device="cuda")  # what the next call's workspace is made of
+        del junk
+        assert torch.equal(ops.paged_attention(*args), want)
+        out.zero_()
+        graph.replay()
+        assert torch.equal(ops.paged_attention(*other), want_other)
+        graph.replay()
+        assert torch.equal(out, want)
