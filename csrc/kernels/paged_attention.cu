@@ -490,6 +490,7 @@ struct Kernel {
             const int n = 2 * (pair ? r.blocks : (r.blocks + 1 - s) / 2);  // half blocks
             // With the same rows in both streams, blocks 2 t and 2 t + 1 are taken together, one by each stream.
             const bool before = !pair && s == 1;
+            const bool early = pair || (L::kKeys >= 4 && r.blocks >= 16);
             wait(&c->q_full[0], n_q[0]++ & 1);
             if (pair && s == 1) wait(&c->q_full[1], n_q[1]++ & 1);
             tmem_fence_after();
@@ -549,11 +550,11 @@ struct Kernel {
                     next_v();
                     if (!pair && s == 0 && i < r.blocks) pass_v();
                 }
-                if (pair) {
+                if (early) {
                     if (i + 2 < n) scores(i + 2);
                 } else if ((i & 1) && i + 1 < n) {
-                    // K of a stream's next block only after V of this one is free: the two streams would otherwise hold
-                    // four tiles, and there would be little room to load ahead
+                    // K of a stream's next block only after V of this one is free: with few tiles in the rings the two
+                    // streams would hold four, and there would be little room to load ahead
                     scores(i + 1);
                     scores(i + 2);
                 }
