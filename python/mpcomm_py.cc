@@ -14,6 +14,7 @@
 #include <cstring>
 #include <optional>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "cuda/gpu.h"
@@ -63,6 +64,15 @@ std::pair<uintptr_t, uintptr_t> kv_span(const kern::KvRowsArgs &a, const kern::K
     return {base, batch > 0 && tokens > 0 && g.heads > 0 ? base + (last + 1) * size : base};
 }
 
+// Whether rows of `n` elements at `a` and of `m` at `b`, both `step` elements apart, lie between each other (heads of
+// one fused projection).
+bool rows_between(const void *a, int64_t n, const void *b, int64_t m, int64_t step, int size) {
+    const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
+    if (step <= 0 || off % size) return false;
+    const int64_t at = ((off / size) % step + step) % step;  // of b's row behind a's
+    return at >= n && at + m <= step;
+}
+
 // A destination is its own source or shares no memory with any source.
 void refuse_overlap(const kern::KvRowsArgs &a, int size) {
     for (int i = 0; i < a.groups; ++i) {
@@ -70,11 +80,36 @@ void refuse_overlap(const kern::KvRowsArgs &a, int size) {
         if (d.plane < 0 && d.src == d.dst && d.sb == d.db && d.st == d.dt && d.sh == d.dh && d.sd == d.dd) continue;
         const auto to = kv_span(a, d, true, size);
         for (int j = 0; j < a.groups; ++j) {
-            const auto from = kv_span(a, a.group[j], false, size);
-            if (to.first < from.second && from.first < to.second)
-                throw py::value_error("a destination overlaps a source that it is not");
+            const kern::KvRowGroup &f = a.group[j];
+            const auto from = kv_span(a, f, false, size);
+            if (to.first >= from.second || from.first >= to.second) continue;
+            if (d.plane < 0 && d.dt == f.st && (a.tokens == a.rows || (d.db == f.sb && f.sb % f.st == 0)) &&
+                rows_between(f.src, (f.heads - 1) * f.sh + (a.dim - 1) * f.sd + 1, d.dst,
+                             (d.heads - 1) * d.dh + (a.dim - 1) * d.dd + 1, f.st, size))
+                continue;
+            throw py::value_error("a destination overlaps a source that it is not");
         }
     }
+}
+
+// The same for attention: the output is the queries themselves, or shares no memory with them or the cache.
+void refuse_overlap(const kern::PagedAttentionArgs &a) {
+    auto span = [](const void *p, int64_t elements) {
+        const auto at = reinterpret_cast<uintptr_t>(p);
+        return std::pair<uintptr_t, uintptr_t>{at, at + static_cast<uintptr_t>(elements) * 2};
+    };
+    auto apart = [](std::pair<uintptr_t, uintptr_t> x, std::pair<uintptr_t, uintptr_t> y) {
+        return x.first >= y.second || y.first >= x.second;
+    };
+    if (a.rows <= 0 || a.batch.pages <= 0) return;
+    const int64_t q_row = (a.q_heads - 1) * a.q_sh + a.dim, o_row = (a.q_heads - 1) * a.o_sh + a.dim;
+    const auto out = span(a.out, (a.rows - 1) * a.o_st + o_row), q = span(a.q, (a.rows - 1) * a.q_st + q_row);
+    const auto pool = span(a.pool, (a.batch.pages - 1) * a.pool_page + a.pool_plane + (a.kv_heads - 1) * a.pool_head +
+                                       (a.batch.page_tokens - 1) * a.pool_token + a.dim);
+    const bool same = a.out == a.q && (a.o_st == a.q_st || a.rows == 1) && (a.o_sh == a.q_sh || a.q_heads == 1);
+    if (!apart(out, pool) ||
+        (!same && !apart(out, q) && !(a.q_st == a.o_st && rows_between(a.q, q_row, a.out, o_row, a.q_st, 2))))
+        throw py::value_error("out overlaps the queries or the cache");
 }
 
 class PyMPComm {
@@ -945,6 +980,7 @@ PYBIND11_MODULE(_mpcomm, m) {
             a.workspace = reinterpret_cast<void *>(workspace);
             a.workspace_bytes = workspace_bytes;
             a.status = reinterpret_cast<uint32_t *>(status);
+            refuse_overlap(a);
             py::gil_scoped_release r;
             return kern::paged_attention(a, dtype, device, reinterpret_cast<void *>(stream));
         },

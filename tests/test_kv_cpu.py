@@ -149,6 +149,35 @@ def test_overlapping_destinations_are_refused():
     for shift in (2, 64, 126, -126):
         with pytest.raises(ValueError):
             call(4096, 4096 + shift)
+    # rows between rows of one buffer, 6 heads wide: heads 0-1 to 2-3 and 4-5 to 0-1 share nothing, 0-1 to 1-2 do
+    wide = (0, 6 * dim, dim, 1)
+    call = lambda src, dst, d=-1: mpcomm._native.kv_rows(  # noqa: E731
+        [(4096 + src * 16, 4096 + dst * 16, *wide, *wide, heads, 1, -1)], dim, 0, False, rows, rows, 0, False, 1.0, 1.0, 0, 0, 0,
+        0, None, 7, d, 0)
+    for src, dst in ((0, 2), (4, 0), (2, 4)):
+        assert call(src, dst) != 0  # goes on to the launch, which has no such type or device here
+    for src, dst in ((0, 1), (1, 0), (4, 5), (5, 0)):
+        with pytest.raises(ValueError):
+            call(src, dst)
+
+
+def test_overlapping_outputs_of_attention_are_refused():
+    import mpcomm
+
+    def call(out, out_strides=(64, 16), q_strides=(64, 16), q=1 << 20, pool=1 << 30):
+        batch = (0, 0, 1, 1, 0, 0, 0, 0, 1, 8, 4)
+        return mpcomm._native.paged_attention(q, *q_strides, out, *out_strides, 0, pool, 512, 256, 128, 16, 4, 4, 2, 16, 1.0,
+                                              True, 0, False, batch, 0, 0, 7, -1, 0)
+
+    q = 1 << 20
+    for fine in (q, q + 512, q - 512, (1 << 30) - 512):
+        assert call(fine) != 0  # on to the launch
+    assert call(q + 128, (128, 16), (128, 16)) != 0  # between the queries' rows
+    for bad in (q + 2, q + 128, q - 128, (1 << 30) - 2, (1 << 30) + 100):
+        with pytest.raises(ValueError):
+            call(bad)
+    with pytest.raises(ValueError):
+        call(q, (64, 16), (128, 16))
 
 
 def test_native_plan():

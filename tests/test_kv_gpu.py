@@ -569,3 +569,44 @@ def test_attention_workspaces_of_any_contents():
         assert torch.equal(ops.paged_attention(*other), want_other)
         graph.replay()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("news", [[1, 1], [70, 3]])
+def test_attention_passes_on_what_is_not_a_number(news):
+    """NaN in a query or in a seen key, and a score of infinity, make their rows NaN, as the formula does, and no other
+    rows of their sequence's earlier tokens or of other sequences."""
+    args, how = _attention_case(news, [300, 200], q_heads=4, kv_heads=2, dim=64, seed=33)
+    q, pool, table, lens, starts = args
+    want, _, tol, _ = ref.attention(*args)
+    q[0, 1, 5] = math.nan
+    got, lse = ops.paged_attention(*args, return_lse=True)
+    assert got[0, 1].isnan().all() and lse[0, 1].isnan()
+    rest = torch.ones(got.shape[:2], dtype=torch.bool, device="cuda")
+    rest[0, 1] = False
+    _near(got[rest], want[rest], tol[rest])
+    q[0, 1, 5] = math.inf
+    assert ops.paged_attention(*args)[0, 1].isnan().all()  # infinite scores of both signs
+    q[0, 1] = 0.0
+    pool[int(table[1, 0]), 0, 1, 3, 0] = math.nan  # a key of the second sequence, seen by all its tokens through heads 2, 3
+    got = ops.paged_attention(*args)
+    assert got[news[0]:, 2:].isnan().all() and not got[:, :2].isnan().any() and not got[:news[0]].isnan().any()
+
+
+def test_append_and_attention_between_the_rows_of_one_buffer():
+    """Queries, keys, values, rotated queries and outputs side by side in one buffer."""
+    args, how = _attention_case([6, 1], [40, 300], q_heads=4, kv_heads=2, dim=64, seed=34)
+    q, pool, table, lens, starts = args
+    freq = ops.rotary_frequencies(64, device="cuda")
+    k, v = _randn(7, 2, 64, seed=35), _randn(7, 2, 64, seed=36)
+    other = pool.clone()
+    _, turned = ops.paged_append(k, v, other, table, lens, starts, inv_freq=freq, q=q)
+    want = ops.paged_attention(turned, other, table, lens, starts)
+    wide = torch.cat((q, k, v, torch.zeros(7, 8, 64, dtype=BF16, device="cuda")), 1)
+    ops.paged_append(wide[:, 4:6], wide[:, 6:8], pool, table, lens, starts, inv_freq=freq, q=wide[:, :4], q_out=wide[:, 8:12])
+    ops.paged_attention(wide[:, 8:12], pool, table, lens, starts, out=wide[:, 12:])
+    assert torch.equal(wide[:, 8:12], turned) and torch.equal(wide[:, 12:], want) and torch.equal(wide[:, :4], q)
+    for bad in (wide[:, 9:13], wide[:, 7:11]):
+        with pytest.raises(ValueError):
+            ops.paged_attention(wide[:, 8:12], pool, table, lens, starts, out=bad)
+    with pytest.raises(ValueError):
+        ops.rotary(wide[:, :4], torch.arange(7, device="cuda"), freq, out=wide[:, 1:5])
