@@ -914,7 +914,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // Joins the tiles that several CTAs share: block (c, y) the one that begins in
-// CTA c and does not end there, the y-th part of its rows.
+// CTA c and does not end there, the y-th part of its rows. A launch of its own
+// that is on its way while the first one ends: joined in the first one, by the
+// warp that finds all parts marked, decode of one sequence took 23 us and not
+// 19, of 32 ragged ones 271 and not 255, since every part then waits until its
+// stores are seen by all.
 constexpr int kJoinThreads = 128;
 template <int DP, typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ KernelArgs g) {
@@ -1051,7 +1055,11 @@ int launch(KernelArgs &g, int dtype, int device, bool join, cudaStream_t st) {
     e = cudaGetLastError();
     if (e != cudaSuccess || !join) return static_cast<int>(e);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(g.ctas, 8);
+    // Blocks for the rows of a tile, two passes of four rows each at most: 256 rows take 32 (against 8: a chunk of 1,024
+    // over 8,192 tokens 152 -> 143 us); where each sequence has one new token a tile has few rows, and idle blocks
+    // would cost 2 us.
+    const int64_t rows = (g.a.rows - g.a.batch.seqs + 1) * g.shape.heads;
+    cfg.gridDim = dim3(g.ctas, static_cast<unsigned>(plan_clamp((rows + 7) / 8, 4, 32)));
     cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr;
