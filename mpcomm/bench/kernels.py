@@ -18,6 +18,12 @@ Cases (inputs larger than the 126 MB L2 where DRAM/PCIe traffic matters):
                            local buffers, 512 x 64 KiB pages
   nvls                     multimem broadcast through a 1-GPU multicast object
   wait_flag                bounded flag wait on a flag that is already set
+  rotary                   rotary positions of 8,192 x 32 heads x 128, bf16
+  append                   4,096 tokens' keys and values into a paged cache,
+                           keys and queries rotated on the way
+  attention_decode         one token of 32 sequences of 4,096 (GB/s of K and V)
+  attention_chunk          1,024 tokens of one sequence of 8,192 (TFLOP/s beside
+                           the GB/s)
 With --time each case is also timed with CUDA events (after 2 warm-ups) and
 its GB/s printed as one JSON line.
 """
@@ -32,10 +38,13 @@ import torch
 
 import mpcomm
 from mpcomm import ops
+from mpcomm.models import LLAMA3_8B_KV
 
 PAGE = 65536
 ALL = ["gather_tma", "gather_sm", "gather_1k", "scatter_1k", "scatter_tma", "copy_d2d", "copy_h2d", "crc32", "crc32_noalloc",
-       "pxn_local", "fanout_local", "gather_bcast_p2p", "nvls", "wait_flag"]
+       "pxn_local", "fanout_local", "gather_bcast_p2p", "nvls", "wait_flag", "rotary", "append", "attention_decode",
+       "attention_chunk"]
+CHUNK_FLOPS = 4 * 32 * 128 * sum(range(8192 - 1024 + 1, 8192 + 1))  # of attention_chunk: pairs that are seen
 
 
 def build_cases():
@@ -80,8 +89,36 @@ def build_cases():
                              512 * PAGE),
         "wait_flag": (lambda: ops.wait_flag(flag.data_ptr(), 1, 1_000_000, status.data_ptr()), 8),
     }
-    keep = (pool, idx, out, big, big2, host, crc_out, flag, status, ctr, pool1k, idx1k, out1k)
+    kv_cases, kv_keep = build_kv_cases()
+    cases.update(kv_cases)
+    keep = (kv_keep, pool, idx, out, big, big2, host, crc_out, flag, status, ctr, pool1k, idx1k, out1k)
     return cases, keep
+
+
+def build_kv_cases():
+    """Rotary positions, appending to a paged cache and attention over it, on Llama-3-8B pages."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    heads, kv_heads, dim, page = 32, LLAMA3_8B_KV.kv_heads, LLAMA3_8B_KV.head_dim, LLAMA3_8B_KV.page_tokens
+    bytes_pool = torch.empty((32 * 4096 // page, LLAMA3_8B_KV.page_bytes), dtype=torch.uint8, device="cuda")
+    cache = LLAMA3_8B_KV.as_cache(bytes_pool)
+    cache.normal_(generator=g)
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pages = torch.randperm(cache.shape[0], generator=g, device="cuda", dtype=torch.int32)
+    many = (cache, pages.view(32, -1), ints([4096] * 32), ints(range(33)))
+    one = (cache, pages[:512].view(1, -1), ints([8192]), ints([0, 1024]))
+    prompt = (cache, pages[:256].view(1, -1), ints([4096]), ints([0, 4096]))
+    qkv = torch.randn((8192, heads + 2 * kv_heads, dim), generator=g, device="cuda", dtype=torch.bfloat16)
+    q, k, v = qkv[:4096, :heads], qkv[:4096, heads:heads + kv_heads], qkv[:4096, heads + kv_heads:]
+    x = torch.randn((8192, heads, dim), generator=g, device="cuda", dtype=torch.bfloat16)
+    out, positions, freq = torch.empty_like(x), torch.arange(8192, device="cuda"), ops.rotary_frequencies(dim, 500000.0, device="cuda")
+    token = 2 * kv_heads * dim * 2  # bytes of a token's keys and values
+    cases = {
+        "rotary": (lambda: ops.rotary(x, positions, freq, out=out), 2 * x.numel() * 2),
+        "append": (lambda: ops.paged_append(k, v, *prompt, inv_freq=freq, q=q, q_out=out[:4096]), 2 * 4096 * qkv[0].numel() * 2),
+        "attention_decode": (lambda: ops.paged_attention(q[:32], *many, out=out[:32]), 32 * 4096 * token),
+        "attention_chunk": (lambda: ops.paged_attention(q[:1024], *one, out=out[:1024]), 8192 * token + 2 * 1024 * heads * dim * 2),
+    }
+    return cases, (cache, qkv, x, out)
 
 
 def nvls_case():
@@ -129,7 +166,8 @@ def main(argv=None):
             e1.record()
             torch.cuda.synchronize()
             ms = e0.elapsed_time(e1) / a.iters
-            print(json.dumps({"case": name, "ms": round(ms, 4), "gbs": round(nbytes / (ms * 1e-3) / 1e9, 2)}),
+            more = {"tflops": round(CHUNK_FLOPS / (ms * 1e-3) / 1e12, 1)} if name == "attention_chunk" else {}
+            print(json.dumps({"case": name, "ms": round(ms, 4), "gbs": round(nbytes / (ms * 1e-3) / 1e9, 2), **more}),
                   flush=True)
     if "nvls" in cases:
         keep[-1][0].close()
