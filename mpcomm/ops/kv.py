@@ -97,9 +97,17 @@ def _stream(stream: Optional[torch.cuda.Stream], device: int) -> int:
 def _empty(like: torch.Tensor, shape, dtype, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
     """A new tensor that belongs to the stream it is written on."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=like.device)
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _empty_like(like: torch.Tensor, stream: Optional[torch.cuda.Stream]) -> torch.Tensor:
+    """The same of the shape and type of another, whatever its strides. 1.5 us; torch.empty, given all by name, 3.3."""
+    if stream is None:
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
 def _on_gpu(what: str, device: int) -> None:
@@ -163,9 +171,8 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, x, positions, inv_freq, how):
         ctx.save_for_backward(positions, inv_freq)
         ctx.how = how
-        shape = x.shape
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-        return out if 0 in shape else _turn(x, positions, inv_freq, *how, out, None)
+        out = _empty_like(x, None)
+        return out if 0 in x.shape else _turn(x, positions, inv_freq, *how, out, None)
 
     @staticmethod
     def backward(ctx, grad):
@@ -174,9 +181,8 @@ class _Rotary(torch.autograd.Function):
         interleaved, magnitude, sign = ctx.how
         if grad.requires_grad and torch.is_grad_enabled():
             return _Rotary.apply(grad, positions, inv_freq, (interleaved, magnitude, -sign)), None, None, None
-        shape = grad.shape
-        out = torch.empty(shape, dtype=grad.dtype, device=grad.device)
-        if 0 not in shape:
+        out = _empty_like(grad, None)
+        if 0 not in grad.shape:
             _turn(grad, positions, inv_freq, interleaved, magnitude, -sign, out, None)
         return out, None, None, None
 
@@ -210,7 +216,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
         return _Rotary.apply(x, positions, inv_freq, (bool(interleaved), float(magnitude), 1.0))
     if out is None:
         _on_gpu("rotary", device)
-        out = _empty(x, shape, x.dtype, stream)
+        out = _empty_like(x, stream)
     else:
         if out.shape != shape or out.dtype != x.dtype or out.get_device() != device:
             raise ValueError("out must have the shape, type and device of x")
@@ -316,7 +322,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
             raise ValueError("q must have the tokens of k")
         if q_out is None:
             _on_gpu("paged_append", device)
-            q_out = _empty(q, q_shape, q.dtype, stream)
+            q_out = _empty_like(q, stream)
         else:
             if _rows(q_out, "q_out", pool, dim, device) != q_shape:
                 raise ValueError("q_out must have the shape of q")
@@ -374,7 +380,7 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     fresh = out is None
     if fresh:
         _on_gpu("paged_attention", device)
-        out = _empty(q, shape, q.dtype, stream)
+        out = _empty_like(q, stream)
     else:
         if _rows(out, "out", pool, dim, device) != shape:
             raise ValueError("out must have the shape of q")
