@@ -581,21 +581,28 @@ struct Kernel {
         return r;
     }
 
-    // Replaces the scores of columns outside [lo, hi) and on boxes that are not there; the first column is key
-    // `at` of its block.
-    __device__ __forceinline__ void mask_scores(uint32_t (&x)[2][32], int lo, int hi, int at, uint32_t boxes) const {
+    // Replaces, in tensor memory, a half block's scores of columns outside [lo, hi) and on boxes that are not there;
+    // its first column is key `at` of its block. Few blocks need it, so it is little code away from the loop's:
+    // fetching instructions that run once a tile is what costs here. A way through them on registers, with a copy of
+    // the loop's step, took 3 us a tile more (windows of 512 tokens, 8 x 777 new tokens: 99 us, this 85).
+    __device__ __forceinline__ void mask_scores(uint32_t ts, int lo, int hi, int at, uint32_t boxes) const {
         const int shift = 7 - g.box_shift;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int up = hi - j * 32, down = lo - j * 32;
+#pragma unroll 1
+        for (int j = 0; j < kHalfKeys; j += 32) {
+            const int up = hi - j, down = lo - j;
             uint32_t seen = up >= 32 ? ~0u : up <= 0 ? 0u : (1u << up) - 1;
             if (down > 0) seen = down >= 32 ? 0u : seen & (~0u << down);
             if (boxes != ~0u)
-                for (int e = 0; e < 32; ++e) seen &= ~((~boxes >> ((at + j * 32 + e) >> shift) & 1u) << e);
+                for (int e = 0; e < 32; ++e) seen &= ~((~boxes >> ((at + j + e) >> shift) & 1u) << e);
+            uint32_t x[32];
+            tmem_ld32(ts + j, x);
+            tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-                if (!(seen >> e & 1u)) x[j][e] = 0xff800000u;
+                if (!(seen >> e & 1u)) x[e] = 0xff800000u;
+            tmem_st32(ts + j, x);
         }
+        tmem_wait_st();
     }
 
     // The largest of a row's 64 scores, by four chains; NaN if one is.
@@ -667,8 +674,7 @@ struct Kernel {
             const int all_lo = __reduce_max_sync(~0u, lo), all_hi = __reduce_min_sync(~0u, hi);
             // m, the reference, is ref * scale, rounded; a weight is 2^(x * times + less).
             float m = -INFINITY, ref = 0.f, times = scale, less = 0.f, sum = 0.f;
-            // A half block from its scores to its weights. Masked ones are rare and have code of their own, away from
-            // the loop's: the instructions that a step goes past cost it as much as some that it executes.
+            // A half block from its scores to its weights.
             auto step = [&](int i, uint32_t ts, uint32_t (&x)[2][32]) {
                 const float top = largest(x), next = top * scale;
                 const bool move = !(next <= m + kRescale);  // NaN moves it too
@@ -737,17 +743,14 @@ struct Kernel {
                     }
                     continue;
                 }
+                const uint32_t boxes = c->mask[(n_block + block) % kMaskSlots];
+                if (__builtin_expect(all_hi < key0 + kHalfKeys || all_lo > key0 || boxes != ~0u, 0))
+                    mask_scores(ts, lo - key0, hi - key0, half * kHalfKeys, boxes);
                 uint32_t x[2][32];
                 tmem_ld32(ts, x[0]);
                 tmem_ld32(ts + 32, x[1]);
-                const uint32_t boxes = c->mask[(n_block + block) % kMaskSlots];
                 tmem_wait_ld();
-                if (__builtin_expect(all_hi >= key0 + kHalfKeys && all_lo <= key0 && boxes == ~0u, 1)) {
-                    step(i, ts, x);
-                } else {
-                    mask_scores(x, lo - key0, hi - key0, half * kHalfKeys, boxes);
-                    step(i, ts, x);
-                }
+                step(i, ts, x);
             }
             n_block += r.blocks;
             if (steps) {
