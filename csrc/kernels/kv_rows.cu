@@ -9,6 +9,12 @@
 // -t. The angle is reduced in 64 bits (a position of 2^20 at one radian each
 // would be off by 2^-4 radians in 32), in turns, so that the reduction is one
 // rint(); sine, cosine and the products are 32-bit, rounded once to the type.
+//
+// Bound by memory: each element is read and written once. 8,192 x 32 heads x
+// 128 in bf16, 134 MB, take 29 us (4.6 TB/s, of 6.55 that a copy of gigabytes
+// reaches); 4,096 tokens of 8 heads' keys and values into 64 KiB pages with 32
+// heads' queries beside them, 101 MB, 24 us. Few tokens take what a launch
+// does.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -127,7 +133,7 @@ struct RowsShape {
 // then a lane of the block's (row, head) pairs. A thread holds its first
 // pair's elements before the rows' places, sines and cosines are known, and
 // always those of the next pair while it turns and stores one, so that the
-// trips to memory overlap. A block's sines and cosines are computed once for
+// trips to memory overlap (two pairs ahead: 3 % slower). A block's sines and cosines are computed once for
 // all heads. N > 1 needs unit element strides, 16-byte aligned bases and
 // strides and pairs, dim multiples of N (of N / 2 for interleaved pairs).
 template <typename T, int N, bool INTERLEAVED, bool PAGED>

@@ -33,6 +33,14 @@
 // page that is none) are read as zeros: their boxes are put outside the pool,
 // where the TMA fills zeros. So nothing that lies there reaches a result, and
 // a masked score is replaced, never added to.
+//
+// What bounds it: single tokens, reading K and V (32 sequences of 4,096, 537
+// MB: 97 us, 5.5 TB/s; the products are done for 128 rows, most of them
+// unused, and keep the tensor pipe busy for a third of that). Chunks, the chain
+// of a half block's scores, exponentials and products, of which two overlap:
+// 1,024 tokens over 8,192 take 133 us (969 TFLOP/s), 4,096 over 16,384 take
+// 808 (1.19 PFLOP/s; a library product reaches 1.66 in a burst, 1.38 when it
+// runs for seconds).
 #include <atomic>
 #include <cstring>
 

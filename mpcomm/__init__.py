@@ -8,7 +8,8 @@ helpers (reference python/__init__.py:47-93).
 
 Subpackages:
   * ``mpcomm.ops``      tensor-level wrappers of the sm_100a kernels
-                        (paged gather/scatter, CRC32, PXN forward, NVLS).
+                        (paged gather/scatter, CRC32, PXN forward, NVLS;
+                        rotary, append and attention on paged KV caches).
   * ``mpcomm.parallel`` multi-process plumbing: torch.distributed bootstrap,
                         CUDA IPC handle exchange, NVLS multicast groups.
   * ``mpcomm.models``   workload shapes the benchmarks use (Llama-3-8B paged
