@@ -27,7 +27,9 @@
 // Weights are rounded to the cache's type for the second product; sums,
 // maxima, scores and outputs are 32-bit. m only moves when a score passes it
 // by 2^8 (kRescale), so O_s is hardly ever rescaled; the weights then reach
-// 2^8, which both types hold with the same relative precision.
+// 2^8, which both types hold with the same relative precision. In fp16 those
+// below 2^-14 have a step of 2^-24 (off by at most 2^-25 of the reference each),
+// as outputs below 2^-14 have.
 //
 // Keys that no row of a tile sees (behind a sequence, before a window, on a
 // page that is none) are read as zeros: their boxes are put outside the pool,
