@@ -24,12 +24,15 @@
 //   warps 9, 10     issue the matrix instructions of stream 0, 1
 //   warp 11         loads the queries and V blocks
 //
-// Weights are rounded to the cache's type for the second product; sums,
-// maxima, scores and outputs are 32-bit. m only moves when a score passes it
-// by 2^8 (kRescale), so O_s is hardly ever rescaled; the weights then reach
-// 2^8, which both types hold with the same relative precision. In fp16 those
-// below 2^-14 have a step of 2^-24 (off by at most 2^-25 of the reference each),
-// as outputs below 2^-14 have.
+// Weights are rounded to the cache's type for the second product, whose two
+// operands have one type; sums, maxima, scores and outputs are 32-bit. m only
+// moves when a score passes the one it was taken from by 2^8 (kRescale), so
+// O_s is hardly ever rescaled. In bf16 m is that score and weights reach 2^8.
+// In fp16 weights below 2^-14 have a step of 2^-24, so m is taken 2^7 lower
+// (kDepth): weights reach 2^15 of the 65,504 that the type holds, and each is
+// off by at most 2^-25 where the largest is at least 2^7, 2^-32 of it. (With m
+// at the score, 8,191 keys 25.2 powers of two below one other lost half of
+// their share.) Outputs below 2^-14 have fp16's step of 2^-24 in any case.
 //
 // Keys that no row of a tile sees (behind a sequence, before a window, on a
 // page that is none) are read as zeros: their boxes are put outside the pool,
@@ -65,6 +68,7 @@ constexpr int kRunSlots = 4;
 constexpr int kFewTiles = 4;  // of a sequence, that one lane counts
 constexpr int kMaskSlots = 16;  // blocks whose masks are kept: more than are ever in flight
 constexpr float kRescale = 8.f;
+constexpr float kFp16Depth = 7.f;
 
 __device__ uint32_t g_attention_status;
 
@@ -158,6 +162,9 @@ struct Kernel {
     static __device__ __forceinline__ uint32_t s_at(int s, int half) { return s * 128 + half * 64; }
     static __device__ __forceinline__ uint32_t o_at(int s) { return 256 + s * DP; }
     static constexpr bool kBf16Type = std::is_same_v<T, __nv_bfloat16>;
+    // powers of two that a row's reference lies below the score it was taken from
+    static constexpr float kDepth = kBf16Type ? 0.f : kFp16Depth;
+    static_assert(kBf16Type || kRescale + kFp16Depth < 16.f, "weights in fp16");
 
     const KernelArgs &g;
     char *smem;
@@ -682,21 +689,21 @@ struct Kernel {
             }
             // keys that every row of the warp sees: blocks inside need no mask
             const int all_lo = __reduce_max_sync(~0u, lo), all_hi = __reduce_min_sync(~0u, hi);
-            // m, the reference, is ref * scale, rounded; a weight is 2^(x * times + less).
+            // m, the reference, is ref * scale - kDepth, rounded; a weight is 2^(x * times + less).
             float m = -INFINITY, ref = 0.f, times = scale, less = 0.f, sum = 0.f;
             // A half block from its scores to its weights.
             auto step = [&](int i, uint32_t ts, uint32_t (&x)[2][32]) {
                 const float top = largest(x), next = top * scale;
-                const bool move = !(next <= m + kRescale);  // NaN moves it too
+                const bool move = !(next <= m + (kRescale + kDepth));  // NaN moves it too
                 if (__builtin_expect(__any_sync(~0u, move && live), 0)) {
                     const float was = m;
                     if (move) {
-                        m = next;
+                        const bool far = fabsf(next) > 0x1p26f;
+                        m = far ? next : next - kDepth;
                         ref = top;
                         // What m was rounded by is the same for the whole row and cancels. Where it could be many
                         // powers of two (the lowest value of a type as a score) the scores are taken times a power of
                         // two instead, which rounds nothing: equal scores have equal weights, and others none.
-                        const bool far = fabsf(m) > 0x1p26f;
                         times = far ? __uint_as_float(__float_as_uint(scale) & 0x7f800000u) : scale;
                         // the weights of a row with a NaN or an infinite score are NaN; nothing seen yet: zero
                         less = m == -INFINITY ? 0.f : m == INFINITY ? NAN : far ? -ref * times : -m;

@@ -610,3 +610,28 @@ def test_append_and_attention_between_the_rows_of_one_buffer():
             ops.paged_attention(wide[:, 8:12], pool, table, lens, starts, out=bad)
     with pytest.raises(ValueError):
         ops.rotary(wide[:, :4], torch.arange(7, device="cuda"), freq, out=wide[:, 1:5])
+
+
+@pytest.mark.parametrize("hot", [0, 4000, 8191])
+@pytest.mark.parametrize("seqs,new", [(160, 1), (80, 256)])
+def test_attention_in_fp16_keeps_many_small_weights(hot, seqs, new):
+    """8,191 keys 25.2 powers of two below one other: their values are all that most of the output has. Enough
+    sequences that a CTA reads a long run of keys against one reference.
+
+    The weights are rounded with a step of 2^-24, off by 2^-25 each, where the largest is at least 2^7: n 2^-32 of the
+    largest value for n keys. The output's own step below 2^-14 is 2^-24."""
+    dim, length, page = 64, 8192, 128
+    pool = torch.zeros(length // page, 2, 1, page, dim, dtype=FP16, device="cuda")
+    pool[:, 1, :, :, 1:] = 1.0
+    at = pool[hot // page, :, 0, hot % page]
+    at[0, 0], at[1, 1:], at[1, 0] = 1.0, 0.0, 1.0
+    q = torch.zeros(seqs * new, 1, dim, dtype=FP16, device="cuda")
+    q[..., 0] = 17.5
+    table = torch.arange(length // page, dtype=torch.int32, device="cuda").expand(seqs, -1).contiguous()
+    lens = torch.full((seqs,), length, dtype=torch.int32, device="cuda")
+    starts = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * new
+    one, one_lse, tol, ltol = ref.attention(q[:1], pool, table[:1], lens[:1], starts[:2].clamp(max=1), scale=1.0, causal=False)
+    got, lse = ops.paged_attention(q, pool, table, lens, starts, scale=1.0, causal=False, return_lse=True)
+    off = length * 2.0 ** -32 + 2.0 ** -25
+    _near(got, one.expand_as(got), (tol + off).expand_as(got), "out")
+    _near(lse, one_lse.expand_as(lse), ltol.expand_as(lse), "lse")
