@@ -34,6 +34,7 @@ struct PlanSeq {
     int first = 0;               // position of the first new token (may be negative)
     int end = 0;                 // keys there are
     int tiles = 0;
+    bool cut = false;            // new tokens see keys that the page table has no room for
 };
 
 struct PlanTile {
@@ -68,6 +69,7 @@ MPCOMM_HD inline PlanSeq plan_seq(const PlanShape &s, int64_t start, int64_t sto
     const int n = plan_clamp(len, 0, kMostTokens);
     q.first = n - q.new_tokens;
     q.end = n < s.tokens ? n : s.tokens;
+    q.cut = q.new_tokens > 0 && len > s.tokens;  // the last one sees itself, whatever the mask
     const int both = 2 * s.tokens_stream;
     q.tiles = q.new_tokens / both + (q.new_tokens % both > 0);
     return q;

@@ -219,6 +219,7 @@ struct Kernel {
         auto count = [&](int b) {
             PlanSeq q;
             if (b < k.seqs) q = sequence(b);
+            if (q.cut && blockIdx.x == 0) atomicOr(status(), kStatusBadIndex);
             int64_t own = q.tiles <= kFewTiles ? plan_part_units(s, q) : 0;
             for (uint32_t many = __ballot_sync(~0u, q.tiles > kFewTiles); many; many &= many - 1) {
                 const int l = __ffs(many) - 1;

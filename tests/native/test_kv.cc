@@ -166,10 +166,30 @@ static void test_plan() {
     }
 }
 
+// A sequence whose keys go past the columns of the page table, or past a length that positions can have, is marked
+// where it has new tokens, and is as long as the table has room for.
+static void test_cut() {
+    PlanShape s;
+    s.rows = 10;
+    for (int tokens : {0, 64, kMostTokens})
+        for (int64_t len : {int64_t{0}, int64_t{1}, int64_t{64}, int64_t{65}, int64_t{kMostTokens}, int64_t{kMostTokens} + 1, INT64_MAX, int64_t{-5}})
+            for (int64_t news : {0, 1, 3})
+                for (int causal : {0, 1}) {
+                    s.tokens = tokens;
+                    s.causal = causal;
+                    const PlanSeq q = plan_seq(s, 2, 2 + news, len);
+                    CHECK(q.cut == (news > 0 && len > tokens));
+                    CHECK(q.end <= tokens && (q.cut || len < 0 || q.end == len || news == 0));
+                }
+    s.tokens = 64;
+    CHECK(!plan_seq(s, 10, 12, 100).cut && !plan_seq(s, 5, 3, 100).cut);  // rows that there are not
+}
+
 int main() {
     test_places();
     test_div();
     test_plan();
+    test_cut();
     std::printf("ok: %ld checks\n", g_checks);
     return 0;
 }

@@ -635,3 +635,31 @@ def test_attention_in_fp16_keeps_many_small_weights(hot, seqs, new):
     off = length * 2.0 ** -32 + 2.0 ** -25
     _near(got, one.expand_as(got), (tol + off).expand_as(got), "out")
     _near(lse, one_lse.expand_as(lse), ltol.expand_as(lse), "lse")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_says_when_a_table_is_too_narrow_or_the_pool_empty(causal):
+    """Keys behind the table's last column, and those of a pool without pages, are not seen: bit 2, as of a bad page."""
+    args, _ = _attention_case([1, 3], [200, 40], dim=64, seed=40)
+    q, pool, table, lens, starts = args
+    status, room = torch.zeros(1, dtype=torch.int32, device="cuda"), table.shape[1] * 16
+
+    def run(*call):
+        status.zero_()
+        got = ops.paged_attention(*call, causal=causal, status_ptr=status.data_ptr())
+        return got, status.item()
+
+    for length, want_status in ((room, 0), (room + 1, 4), (5000, 4), (1 << 30, 4)):
+        lens[0] = length
+        want, _, tol, _ = ref.attention(q, pool, table, lens.clamp(max=5000), starts, causal=causal)
+        got, bits = run(*args)
+        _near(got, want, tol)
+        assert bits == want_status, length
+    wide = lens.long()
+    wide[0] = 1 << 40
+    assert run(q, pool, table, wide, starts)[1] == 4
+    none = torch.tensor([0, 0, 4], dtype=torch.int32, device="cuda")  # nothing new in the sequence that is too long
+    assert run(q, pool, table, lens, none)[1] == 0
+    got, bits = run(q, pool[:0], table, lens, none)
+    assert bits == 4 and not got.any()
+    assert run(q, pool[:0], table, lens * 0, none)[1] == 0
