@@ -19,6 +19,7 @@
 
 #include "cuda/gpu.h"
 #include "kernels/kv.h"
+#include "kernels/kv_overlap.h"
 #include "kernels/launch.h"
 #include "mpcomm.h"
 #include "parallel/vmm.h"
@@ -53,62 +54,34 @@ kern::KvBatch kv_batch(const KvBatchTuple &t) {
     return b;
 }
 
-// Bytes [first, second) that a group's source or destination spans.
-std::pair<uintptr_t, uintptr_t> kv_span(const kern::KvRowsArgs &a, const kern::KvRowGroup &g, bool dst, int size) {
-    const bool paged = dst && g.plane >= 0;
-    const int64_t tokens = paged ? a.batch.page_tokens : a.tokens;
-    const int64_t batch = paged ? a.batch.pages : a.rows / (a.tokens > 0 ? a.tokens : 1);
-    const int64_t last = (batch - 1) * (dst ? g.db : g.sb) + (tokens - 1) * (dst ? g.dt : g.st) +
-                         (g.heads - 1) * (dst ? g.dh : g.sh) + (a.dim - 1) * (dst ? g.dd : g.sd);
-    const auto base = reinterpret_cast<uintptr_t>(dst ? g.dst : g.src);
-    return {base, batch > 0 && tokens > 0 && g.heads > 0 ? base + (last + 1) * size : base};
-}
-
-// Whether rows of `n` elements at `a` and of `m` at `b`, both `step` elements apart, lie between each other (heads of
-// one fused projection).
-bool rows_between(const void *a, int64_t n, const void *b, int64_t m, int64_t step, int size) {
-    const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a));
-    if (step <= 0 || off % size) return false;
-    const int64_t at = ((off / size) % step + step) % step;  // of b's row behind a's
-    return at >= n && at + m <= step;
+// What a group reads, or writes (a paged group: anywhere in its plane of the cache).
+kern::StridedSet kv_set(const kern::KvRowsArgs &a, const kern::KvRowGroup &g, bool dst) {
+    const int64_t tokens = a.tokens > 0 ? a.tokens : 1;
+    if (!dst) return {g.src, {{g.sb, a.rows / tokens}, {g.st, a.tokens}, {g.sh, g.heads}, {g.sd, a.dim}}};
+    if (g.plane < 0) return {g.dst, {{g.db, a.rows / tokens}, {g.dt, a.tokens}, {g.dh, g.heads}, {g.dd, a.dim}}};
+    return {g.dst, {{g.db, a.batch.pages}, {g.dt, a.batch.page_tokens}, {g.dh, g.heads}, {g.dd, a.dim}}};
 }
 
 // A destination is its own source or shares no memory with any source.
 void refuse_overlap(const kern::KvRowsArgs &a, int size) {
+    kern::StridedSet from[3], to;
+    for (int i = 0; i < a.groups; ++i) from[i] = kv_set(a, a.group[i], false);
     for (int i = 0; i < a.groups; ++i) {
-        const kern::KvRowGroup &d = a.group[i];
-        if (d.plane < 0 && d.src == d.dst && d.sb == d.db && d.st == d.dt && d.sh == d.dh && d.sd == d.dd) continue;
-        const auto to = kv_span(a, d, true, size);
-        for (int j = 0; j < a.groups; ++j) {
-            const kern::KvRowGroup &f = a.group[j];
-            const auto from = kv_span(a, f, false, size);
-            if (to.first >= from.second || from.first >= to.second) continue;
-            if (d.plane < 0 && d.dt == f.st && (a.tokens == a.rows || (d.db == f.sb && f.sb % f.st == 0)) &&
-                rows_between(f.src, (f.heads - 1) * f.sh + (a.dim - 1) * f.sd + 1, d.dst,
-                             (d.heads - 1) * d.dh + (a.dim - 1) * d.dd + 1, f.st, size))
-                continue;
-            throw py::value_error("a destination overlaps a source that it is not");
-        }
+        to = kv_set(a, a.group[i], true);
+        if (a.group[i].plane < 0 && to == from[i]) continue;
+        for (int j = 0; j < a.groups; ++j)
+            if (kern::sets_overlap(to, from[j], size))
+                throw py::value_error("a destination overlaps a source that it is not");
     }
 }
 
 // The same for attention: the output is the queries themselves, or shares no memory with them or the cache.
 void refuse_overlap(const kern::PagedAttentionArgs &a) {
-    auto span = [](const void *p, int64_t elements) {
-        const auto at = reinterpret_cast<uintptr_t>(p);
-        return std::pair<uintptr_t, uintptr_t>{at, at + static_cast<uintptr_t>(elements) * 2};
-    };
-    auto apart = [](std::pair<uintptr_t, uintptr_t> x, std::pair<uintptr_t, uintptr_t> y) {
-        return x.first >= y.second || y.first >= x.second;
-    };
-    if (a.rows <= 0 || a.batch.pages <= 0) return;
-    const int64_t q_row = (a.q_heads - 1) * a.q_sh + a.dim, o_row = (a.q_heads - 1) * a.o_sh + a.dim;
-    const auto out = span(a.out, (a.rows - 1) * a.o_st + o_row), q = span(a.q, (a.rows - 1) * a.q_st + q_row);
-    const auto pool = span(a.pool, (a.batch.pages - 1) * a.pool_page + a.pool_plane + (a.kv_heads - 1) * a.pool_head +
-                                       (a.batch.page_tokens - 1) * a.pool_token + a.dim);
-    const bool same = a.out == a.q && (a.o_st == a.q_st || a.rows == 1) && (a.o_sh == a.q_sh || a.q_heads == 1);
-    if (!apart(out, pool) ||
-        (!same && !apart(out, q) && !(a.q_st == a.o_st && rows_between(a.q, q_row, a.out, o_row, a.q_st, 2))))
+    const kern::StridedSet out(a.out, {{a.o_st, a.rows}, {a.o_sh, a.q_heads}, {1, a.dim}});
+    const kern::StridedSet q(a.q, {{a.q_st, a.rows}, {a.q_sh, a.q_heads}, {1, a.dim}});
+    const kern::StridedSet pool(a.pool, {{a.pool_page, a.batch.pages}, {a.pool_plane, 2}, {a.pool_head, a.kv_heads},
+                                         {a.pool_token, a.batch.page_tokens}, {1, a.dim}});
+    if (kern::sets_overlap(out, pool, 2) || (!(out == q) && kern::sets_overlap(out, q, 2)))
         throw py::value_error("out overlaps the queries or the cache");
 }
 

@@ -6,10 +6,12 @@
 #include <cstdlib>
 #include <map>
 #include <random>
+#include <set>
 #include <tuple>
 #include <vector>
 
 #include "kernels/attention_plan.h"
+#include "kernels/kv_overlap.h"
 
 using namespace mpcomm::kern;
 
@@ -185,11 +187,60 @@ static void test_cut() {
     CHECK(!plan_seq(s, 10, 12, 100).cut && !plan_seq(s, 5, 3, 100).cut);  // rows that there are not
 }
 
+// Against every byte of both sets.
+static void test_overlap() {
+    std::mt19937 rng(11);
+    auto pick = [&](int lo, int hi) { return lo + static_cast<int>(rng() % (hi - lo + 1)); };
+    auto make = [&](bool nested) {
+        int64_t e[4], s[4], step = 1;
+        for (int k = 3; k >= 0; --k) {
+            e[k] = pick(nested ? 1 : 0, 4);
+            s[k] = pick(0, 9) ? step : 0;
+            step *= e[k] > 0 ? e[k] + pick(0, 2) : 1;
+            if (!nested) s[k] = pick(-3, 12);
+        }
+        return StridedSet(reinterpret_cast<void *>(uintptr_t{1 << 20} + pick(0, 300)),
+                          {{s[0], e[0]}, {s[1], e[1]}, {s[2], e[2]}, {s[3], e[3]}});
+    };
+    auto bytes = [](const StridedSet &a, int size) {
+        std::vector<int64_t> at{static_cast<int64_t>(a.base)};
+        for (int k = 0; k < a.axes; ++k) {
+            const size_t n = at.size();
+            for (int64_t i = 1; i < a.extent[k]; ++i)
+                for (size_t j = 0; j < n; ++j) at.push_back(at[j] + i * a.stride[k] * size);
+        }
+        std::set<int64_t> all;
+        if (!a.empty)
+            for (int64_t p : at)
+                for (int b = 0; b < size; ++b) all.insert(p + b);
+        return all;
+    };
+    int met = 0;
+    for (int t = 0; t < 20000; ++t) {
+        const StridedSet a = make(t % 3), b = make(t % 2);
+        const int size = t % 5 ? 2 : 4;
+        const auto in_a = bytes(a, size), in_b = bytes(b, size);
+        bool meet = false;
+        for (int64_t p : in_a) meet = meet || in_b.count(p);
+        CHECK(sets_overlap(a, b, size) == meet);
+        met += meet;
+    }
+    CHECK(met > 2000 && met < 18000);
+    // large sets are decided by their strides: heads of one projection of 2^20 rows, side by side and one too far
+    const int64_t rows = 1 << 20, heads = 8, dim = 128;
+    auto part = [&](int64_t first) {
+        return StridedSet(reinterpret_cast<void *>((uintptr_t{1} << 40) + first * dim * 2), {{3 * heads * dim, rows}, {dim, heads}, {1, dim}});
+    };
+    CHECK(!sets_overlap(part(0), part(heads), 2) && !sets_overlap(part(2 * heads), part(0), 2) && sets_overlap(part(0), part(heads - 1), 2));
+    CHECK(part(1) == part(1) && !(part(1) == part(2)));
+}
+
 int main() {
     test_places();
     test_div();
     test_plan();
     test_cut();
+    test_overlap();
     std::printf("ok: %ld checks\n", g_checks);
     return 0;
 }

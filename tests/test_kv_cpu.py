@@ -186,3 +186,28 @@ def test_native_plan():
     assert os.path.exists(exe), "native tests not built (run __graft_entry__.build())"
     r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+def test_overlap_of_interleaved_and_degenerate_strides():
+    """Axes of one element, and strides of zero, say nothing about memory; heads and elements may lie between others."""
+    import mpcomm
+
+    def call(dst, to, src=4096, of=None, rows=4, tokens=4, heads=2, dim=8):
+        group = (src, src + dst * 2, *(of or to), *to, heads, 1, -1)
+        return mpcomm._native.kv_rows([group], dim, 0, False, rows, tokens, 0, False, 1.0, 1.0, 0, 0, 0, 0, None, 7, -1, 0)
+
+    for fine in (  # on to the launch, which has no such type or device here
+        {"dst": 0, "to": (0, 16, 8, 1)}, {"dst": 0, "to": (0, 16, 99, 1), "of": (0, 16, 5, 1), "heads": 1},
+        {"dst": 0, "to": (7, 16, 8, 1), "of": (5, 16, 8, 1)},
+        {"dst": 8, "to": (0, 48, 24, 1)}, {"dst": -16, "to": (0, 48, 24, 1)},  # [tokens, heads, 3, dim]
+        {"dst": 32, "to": (0, 8, 64, 1)},  # [heads, 2, tokens, dim]
+        {"dst": 1, "to": (0, 32, 16, 2)},  # every second element
+    ):
+        assert call(**fine) != 0
+    assert call(16, (32, 0, 8, 1), rows=4, tokens=1) != 0  # a batch of single tokens, between each other
+    for tokens in (1, 2, 4):
+        with pytest.raises(ValueError):
+            call(2, (0, 0, 8, 1), tokens=tokens)  # no stride in rows at all
+    for dst, to in ((4, (0, 48, 24, 1)), (24, (0, 48, 24, 1)), (28, (0, 8, 64, 1)), (8, (0, 8, 64, 1)), (2, (0, 32, 16, 2))):
+        with pytest.raises(ValueError):
+            call(dst, to)
