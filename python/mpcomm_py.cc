@@ -62,15 +62,15 @@ kern::StridedSet kv_set(const kern::KvRowsArgs &a, const kern::KvRowGroup &g, bo
     return {g.dst, {{g.db, a.batch.pages}, {g.dt, a.batch.page_tokens}, {g.dh, g.heads}, {g.dd, a.dim}}};
 }
 
-// A destination is its own source or shares no memory with any source.
+// A destination is its own source, and shares no memory with any other.
 void refuse_overlap(const kern::KvRowsArgs &a, int size) {
     kern::StridedSet from[3], to;
     for (int i = 0; i < a.groups; ++i) from[i] = kv_set(a, a.group[i], false);
     for (int i = 0; i < a.groups; ++i) {
         to = kv_set(a, a.group[i], true);
-        if (a.group[i].plane < 0 && to == from[i]) continue;
+        const bool in_place = a.group[i].plane < 0 && to == from[i];
         for (int j = 0; j < a.groups; ++j)
-            if (kern::sets_overlap(to, from[j], size))
+            if (!(in_place && j == i) && kern::sets_overlap(to, from[j], size))
                 throw py::value_error("a destination overlaps a source that it is not");
     }
 }

@@ -211,3 +211,24 @@ def test_overlap_of_interleaved_and_degenerate_strides():
     for dst, to in ((4, (0, 48, 24, 1)), (24, (0, 48, 24, 1)), (28, (0, 8, 64, 1)), (8, (0, 8, 64, 1)), (2, (0, 32, 16, 2))):
         with pytest.raises(ValueError):
             call(dst, to)
+
+
+def test_queries_in_place_that_are_keys_too_are_refused():
+    """Turned in place while they are read as keys or values: what the cache would hold hangs on the order."""
+    import mpcomm
+
+    rows, heads, dim = 4, 2, 8
+    wide = (0, 6 * dim, dim, 1)  # rows of six heads
+
+    def call(k, v, q, q_out):
+        batch = (0, 0, 1, 1, 0, 0, 0, 0, 1, 8, 4)
+        plane = (2 * heads * 8 * dim, dim, 8 * dim, 1)
+        group = lambda src, dst, *how: (4096 + src * dim * 2, dst, *wide, *how)  # noqa: E731
+        groups = [group(k, 1 << 30, *plane, heads, 1, 0), group(v, (1 << 30) + heads * 8 * dim * 2, *plane, heads, 0, 1),
+                  group(q, 4096 + q_out * dim * 2, *wide, heads, 1, -1)]
+        return mpcomm._native.kv_rows(groups, dim, 0, False, rows, rows, 0, False, 1.0, 1.0, 0, 0, 0, 0, batch, 7, -1, 0)
+
+    assert call(2, 4, 0, 0) != 0 and call(2, 4, 4 * 6, 0) != 0  # apart: on to the launch, which has no such type here
+    for k, v, q in ((0, 4, 0), (1, 4, 0), (2, 1, 2), (4, 0, 0)):
+        with pytest.raises(ValueError):
+            call(k, v, q, q)
