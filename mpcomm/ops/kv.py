@@ -280,8 +280,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
 
     With ``inv_freq`` the keys are rotated on the way as :func:`rotary` does, by their places in their sequences or
     by ``positions`` ``[tokens]``. With ``q`` ``[tokens, q_heads, head_dim]`` the same launch rotates the queries too,
-    into ``q_out`` (``q`` itself, memory apart from ``q``, ``k``, ``v``, or by default a new tensor), and
-    ``(pool, q_out)`` is returned; padding rows of ``q_out`` stay as they were, in a new tensor undefined.
+    into ``q_out`` (``q`` itself, memory apart from ``q``, or by default a new tensor; apart from ``k``, ``v`` and the
+    cache), and ``(pool, q_out)`` is returned; padding rows of ``q_out`` stay as they were, in a new tensor undefined.
 
     ``pool`` is device memory or pinned host memory. A token whose column is behind the page table's width, whose
     page is outside the pool, or that lies before its sequence (``seq_lens[b]`` below its new tokens) stores nothing

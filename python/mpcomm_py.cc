@@ -62,16 +62,18 @@ kern::StridedSet kv_set(const kern::KvRowsArgs &a, const kern::KvRowGroup &g, bo
     return {g.dst, {{g.db, a.batch.pages}, {g.dt, a.batch.page_tokens}, {g.dh, g.heads}, {g.dd, a.dim}}};
 }
 
-// A destination is its own source, and shares no memory with any other.
+// A destination is its own source, and shares no memory with any other; rows and the cache share none either.
 void refuse_overlap(const kern::KvRowsArgs &a, int size) {
-    kern::StridedSet from[3], to;
-    for (int i = 0; i < a.groups; ++i) from[i] = kv_set(a, a.group[i], false);
+    kern::StridedSet from[3], to[3];
+    for (int i = 0; i < a.groups; ++i) from[i] = kv_set(a, a.group[i], false), to[i] = kv_set(a, a.group[i], true);
     for (int i = 0; i < a.groups; ++i) {
-        to = kv_set(a, a.group[i], true);
-        const bool in_place = a.group[i].plane < 0 && to == from[i];
-        for (int j = 0; j < a.groups; ++j)
-            if (!(in_place && j == i) && kern::sets_overlap(to, from[j], size))
+        const bool in_place = a.group[i].plane < 0 && to[i] == from[i];
+        for (int j = 0; j < a.groups; ++j) {
+            if (!(in_place && j == i) && kern::sets_overlap(to[i], from[j], size))
                 throw py::value_error("a destination overlaps a source that it is not");
+            if (a.group[i].plane < 0 && a.group[j].plane >= 0 && kern::sets_overlap(to[i], to[j], size))
+                throw py::value_error("q_out overlaps the cache");
+        }
     }
 }
 

@@ -232,3 +232,24 @@ def test_queries_in_place_that_are_keys_too_are_refused():
     for k, v, q in ((0, 4, 0), (1, 4, 0), (2, 1, 2), (4, 0, 0)):
         with pytest.raises(ValueError):
             call(k, v, q, q)
+
+
+def test_rotated_queries_in_the_cache_are_refused():
+    """Both are written by one launch, in no order."""
+    import mpcomm
+
+    rows, heads, dim, pages, cache = 4, 2, 8, 4, 1 << 30
+    row, plane = (0, heads * dim, dim, 1), (2 * heads * 8 * dim * 2, dim, 8 * dim, 1)  # pages twice as far apart as they are long
+
+    def call(q_out):
+        batch = (0, 0, 1, 1, 0, 0, 0, 0, 1, 8, pages)
+        groups = [(4096, cache, *row, *plane, heads, 1, 0), (8192, cache + heads * 8 * dim * 2, *row, *plane, heads, 0, 1),
+                  (1 << 20, q_out, *row, *row, heads, 1, -1)]
+        return mpcomm._native.kv_rows(groups, dim, 0, False, rows, rows, 0, False, 1.0, 1.0, 0, 0, 0, 0, batch, 7, -1, 0)
+
+    page = plane[0] * 2
+    for fine in (1 << 20, cache - rows * heads * dim * 2, cache + page // 2, cache + page * pages):
+        assert call(fine) != 0  # on to the launch, which has no such type or device here
+    for bad in (cache, cache - 2, cache + page // 2 - 2, cache + page - 2):
+        with pytest.raises(ValueError):
+            call(bad)
