@@ -89,6 +89,8 @@ struct KvRowGroup {
     int plane = -1;
 };
 
+constexpr int kMostHeads = 1 << 30;  // of a row: a block's (row, head) pairs are counted in 32 bits
+
 struct KvRowsArgs {
     KvRowGroup group[3];
     int groups = 0;

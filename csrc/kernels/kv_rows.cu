@@ -279,6 +279,7 @@ int launch_rows(const KvRowsArgs &a, int sms, cudaStream_t st) {
     if (fit < 1 || parts > 65535) return cudaErrorInvalidValue;
     if (rows > fit) rows = fit;
     if (rows > kMaxRowsPerCta) rows = kMaxRowsPerCta;
+    if (rows > kMostHeads / a.heads) rows = kMostHeads / a.heads;
     int64_t lanes = kRowThreads / units;
     if (lanes > rows * a.heads) lanes = rows * a.heads;
     const int64_t ctas = (a.rows + rows - 1) / rows;
@@ -323,7 +324,7 @@ int launch_typed(const KvRowsArgs &a, int sms, cudaStream_t st) {
 int kv_rows(const KvRowsArgs &args, int dtype, int device, void *stream) {
     KvRowsArgs a = args;
     if (a.rows <= 0 || a.heads <= 0 || a.dim <= 0) return 0;
-    if (a.rows > 0x7fffffff || a.tokens <= 0 || a.tokens > a.rows || a.groups < 1 || a.groups > 3 || (!a.in_batch && a.groups > 1))
+    if (a.rows > 0x7fffffff || a.heads > kMostHeads || a.tokens <= 0 || a.tokens > a.rows || a.groups < 1 || a.groups > 3 || (!a.in_batch && a.groups > 1))
         return cudaErrorInvalidValue;
     join_batch(&a);
     DeviceScope on(device);

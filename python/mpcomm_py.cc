@@ -890,7 +890,10 @@ PYBIND11_MODULE(_mpcomm, m) {
            uintptr_t stream, uintptr_t status) {
             kern::KvRowsArgs a;
             if (groups.empty() || groups.size() > 3) throw py::value_error("kv_rows takes one to three groups");
+            int64_t heads = 0;
             for (const auto &g : groups) {
+                heads += g[10];
+                if (g[10] < 0 || heads > kern::kMostHeads) throw py::value_error("a row has more than 2^30 heads");
                 kern::KvRowGroup &q = a.group[a.groups++];
                 q.src = reinterpret_cast<const void *>(g[0]);
                 q.dst = reinterpret_cast<void *>(g[1]);

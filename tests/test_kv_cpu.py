@@ -253,3 +253,16 @@ def test_rotated_queries_in_the_cache_are_refused():
     for bad in (cache, cache - 2, cache + page // 2 - 2, cache + page - 2):
         with pytest.raises(ValueError):
             call(bad)
+
+
+def test_more_heads_than_can_be_counted_are_refused():
+    import mpcomm
+
+    def call(*heads):
+        groups = [(4096, 1 << 50, 0, 4, 2, 1, 0, 4, 2, 1, h, 1, -1) for h in heads]
+        return mpcomm._native.kv_rows(groups, 2, 0, False, 1, 1, 0, False, 1.0, 1.0, 0, 0, 0, 0, None, 7, -1, 0)
+
+    assert call(1 << 30) != 0  # on to the launch, which has no such type or device here
+    for bad in ((1 << 31,), ((1 << 30) + 1,), (1 << 32,), (-1,), (1 << 29, 1 << 29, 1), (1 << 62, 1 << 62)):
+        with pytest.raises(ValueError):
+            call(*bad)
