@@ -78,7 +78,9 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "n
 # A call of a few tokens is over on the GPU in microseconds, so the checks below read each tensor's shape, strides and
 # device once, and compare plain integers.
 
-_current_stream = torch._C._cuda_getCurrentRawStream  # of a device's number
+# Of a device's number: the raw handle, without a Stream object. A torch without CUDA has no such function.
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _check(err: int, what: str) -> None:

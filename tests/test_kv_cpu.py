@@ -2,6 +2,7 @@
 import math
 import os
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -266,3 +267,23 @@ def test_more_heads_than_can_be_counted_are_refused():
     for bad in ((1 << 31,), ((1 << 30) + 1,), (1 << 32,), (-1,), (1 << 29, 1 << 29, 1), (1 << 62, 1 << 62)):
         with pytest.raises(ValueError):
             call(*bad)
+
+
+def test_import_on_a_torch_without_cuda():
+    """What runs on the host loads and runs there; the operators refuse."""
+    code = """
+import torch
+for name in [n for n in dir(torch._C) if n.startswith("_cuda")]:
+    delattr(torch._C, name)
+from mpcomm import ops
+assert ops.crc32_host(b"123456789") == 0xCBF43926
+try:
+    ops.rotary(torch.zeros(1, 1, 2), torch.zeros(1, dtype=torch.int64), ops.rotary_frequencies(2))
+except ValueError as e:
+    assert "runs on CUDA tensors" in str(e)
+else:
+    raise AssertionError("taken")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
+    assert r.returncode == 0, r.stderr[-2000:]
