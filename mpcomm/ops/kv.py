@@ -201,7 +201,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     reduced in 64 bits, so positions may be as far as they like.
 
     ``out`` may be ``x`` itself, or memory apart from it. Differentiable in ``x`` (any number of times) without
-    ``out`` and ``stream``. As with any autograd graph that is captured into a CUDA graph, capture the forward and
+    ``out`` and ``stream``, not in ``inv_freq``: frequencies that require a gradient are refused. As with any autograd graph that is captured into a CUDA graph, capture the forward and
     the backward pass together, and let no eager graph of the same leaves live meanwhile.
     """
     shape, device = x.shape, x.get_device()
@@ -211,6 +211,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     if positions.shape != shape[:-2] and not (len(shape) == 4 and positions.shape == shape[1:2]):
         raise ValueError(f"positions {tuple(positions.shape)} do not fit x {tuple(shape)}")
     _frequencies(inv_freq, shape[-1], device)
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        _no_gradient("rotary in inv_freq")
     if x.requires_grad and torch.is_grad_enabled():
         if out is not None or stream is not None:
             raise ValueError("rotary has a gradient only without out and stream")
@@ -299,7 +301,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
     if shape[1] != kv_heads or _rows(v, "v", pool, dim, device) != shape:
         raise ValueError(f"k and v must have {kv_heads} heads and the same tokens")
     if (k.requires_grad or v.requires_grad or pool.requires_grad or (q is not None and q.requires_grad)
-            or (q_out is not None and q_out.requires_grad)) and torch.is_grad_enabled():
+            or (q_out is not None and q_out.requires_grad)
+            or (inv_freq is not None and inv_freq.requires_grad)) and torch.is_grad_enabled():
         _no_gradient("paged_append")
     _own_memory(pool, "the cache")
     rows = shape[0]

@@ -287,3 +287,24 @@ else:
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=root)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_no_silent_loss_of_the_gradients_of_frequencies_and_outputs():
+    x, pos, freq = torch.zeros(4, 2, 16), torch.arange(4), ops.rotary_frequencies(16)
+    learned = freq.clone().requires_grad_()
+    q = torch.zeros(4, 4, 16, dtype=BF16)
+    for call in (lambda: ops.rotary(x, pos, learned), lambda: ops.rotary(x.clone().requires_grad_(), pos, learned),
+                 lambda: ops.rotary(x, pos, learned, out=torch.zeros_like(x)), lambda: _call("append", inv_freq=learned),
+                 lambda: _append_q(q, learned), lambda: _append_q(q.clone().requires_grad_(), freq),
+                 lambda: _append_q(q, freq, q_out=q.clone().requires_grad_()),
+                 lambda: _call("attention", out=q.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            _refused(call, for_the_device=True)
+
+
+def _append_q(q, inv_freq, **how):
+    table, lens, starts, pages = ref.batch([3, 1], [20, 9], 8)
+    kv = torch.zeros(4, 2, 16, dtype=BF16)
+    return ops.paged_append(kv, kv, torch.zeros(pages, 2, 2, 8, 16, dtype=BF16), table, lens, starts, inv_freq=inv_freq, q=q, **how)
