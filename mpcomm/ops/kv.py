@@ -22,6 +22,7 @@ import math
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -139,6 +140,15 @@ def _no_gradient(what: str) -> None:
     raise RuntimeError(f"mpcomm {what} has no gradient: call it under torch.no_grad()")
 
 
+def _no_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses forward-mode differentiation, which the kernels would lose. Outside of a dual level (a number of 0 or
+    more, where torch says it) no tensor has a tangent, and looking at none of them saves half a microsecond each."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"mpcomm {what} has no forward-mode gradient")
+
+
 def _own_memory(t: torch.Tensor, what: str) -> None:
     """Refuses a destination two of whose elements share a place."""
     if t.is_contiguous():
@@ -181,6 +191,7 @@ class _Rotary(torch.autograd.Function):
         # the rotation is linear and its transpose is the rotation back, so a gradient of the gradient is one more
         positions, inv_freq = ctx.saved_tensors
         interleaved, magnitude, sign = ctx.how
+        _no_tangents("rotary's gradient", grad)
         if grad.requires_grad and torch.is_grad_enabled():
             return _Rotary.apply(grad, positions, inv_freq, (interleaved, magnitude, -sign)), None, None, None
         out = _empty_like(grad, None)
@@ -201,7 +212,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     reduced in 64 bits, so positions may be as far as they like.
 
     ``out`` may be ``x`` itself, or memory apart from it. Differentiable in ``x`` (any number of times) without
-    ``out`` and ``stream``, not in ``inv_freq``: frequencies that require a gradient are refused. As with any autograd graph that is captured into a CUDA graph, capture the forward and
+    ``out`` and ``stream``, not in ``inv_freq``: frequencies that require a gradient are refused, and so is
+    forward mode. As with any autograd graph that is captured into a CUDA graph, capture the forward and
     the backward pass together, and let no eager graph of the same leaves live meanwhile.
     """
     shape, device = x.shape, x.get_device()
@@ -211,6 +223,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     if positions.shape != shape[:-2] and not (len(shape) == 4 and positions.shape == shape[1:2]):
         raise ValueError(f"positions {tuple(positions.shape)} do not fit x {tuple(shape)}")
     _frequencies(inv_freq, shape[-1], device)
+    _no_tangents("rotary", x, inv_freq, out)
     if inv_freq.requires_grad and torch.is_grad_enabled():
         _no_gradient("rotary in inv_freq")
     if x.requires_grad and torch.is_grad_enabled():
@@ -304,6 +317,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
             or (q_out is not None and q_out.requires_grad)
             or (inv_freq is not None and inv_freq.requires_grad)) and torch.is_grad_enabled():
         _no_gradient("paged_append")
+    _no_tangents("paged_append", k, v, pool, q, q_out, inv_freq)
     _own_memory(pool, "the cache")
     rows = shape[0]
     pairs = freq = wide = 0
@@ -375,6 +389,7 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     rows, q_heads, _ = shape
     if (q.requires_grad or pool.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled():
         _no_gradient("paged_attention")
+    _no_tangents("paged_attention", q, pool, out)
     if q_heads == 0 or q_heads % kv_heads:
         raise ValueError(f"{q_heads} query heads cannot share {kv_heads} key heads")
     if dim % 8 or dim > 128 or page_tokens % 8:

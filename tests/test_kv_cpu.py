@@ -3,6 +3,7 @@ import math
 import os
 import subprocess
 import sys
+import types
 
 import pytest
 import torch
@@ -10,6 +11,7 @@ import torch
 import kv_reference as ref
 from mpcomm import ops
 from mpcomm.models import LLAMA3_8B_KV, KVPoolSpec
+from mpcomm.ops import kv
 
 BF16 = torch.bfloat16
 
@@ -308,3 +310,24 @@ def _append_q(q, inv_freq, **how):
     table, lens, starts, pages = ref.batch([3, 1], [20, 9], 8)
     kv = torch.zeros(4, 2, 16, dtype=BF16)
     return ops.paged_append(kv, kv, torch.zeros(pages, 2, 2, 8, 16, dtype=BF16), table, lens, starts, inv_freq=inv_freq, q=q, **how)
+
+
+def test_no_silent_loss_of_tangents():
+    x, pos, freq = torch.zeros(4, 2, 16), torch.arange(4), ops.rotary_frequencies(16)
+    q = torch.zeros(4, 4, 16, dtype=BF16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = lambda t: torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ops.rotary(dual(x), pos, freq), lambda: ops.rotary(x, pos, dual(freq)),
+                     lambda: ops.rotary(dual(x.clone().requires_grad_()), pos, freq), lambda: ops.rotary(x, pos, freq, out=dual(x)),
+                     lambda: _call("append", k=dual), lambda: _call("append", v=dual), lambda: _call("append", pool=dual),
+                     lambda: _call("append", inv_freq=dual(freq)), lambda: _append_q(dual(q), freq),
+                     lambda: _append_q(q, freq, q_out=dual(q)), lambda: _call("attention", q=dual),
+                     lambda: _call("attention", pool=dual), lambda: _call("attention", out=dual(q))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="no forward-mode gradient"):
+                    call()
+        saved = types.SimpleNamespace(saved_tensors=(pos, freq), how=(False, 1.0, 1.0))
+        with pytest.raises(RuntimeError, match="no forward-mode gradient"):
+            kv._Rotary.backward(saved, dual(x))
+        _refused(lambda: ops.rotary(x, pos, freq), for_the_device=True)  # plain tensors are taken
+        _refused(lambda: _call("attention"), for_the_device=True)
