@@ -14,6 +14,9 @@ in slot ``p % page_tokens`` of page ``page_table[b, p // page_tokens]``. Rows
 behind the last sequence are padding. The three tables are int32 or int64
 device tensors, read by the kernels only: nothing here waits for the GPU, and
 a captured CUDA graph follows what they hold when it is replayed.
+
+Tensors that a call writes and the caller gave (``out``, ``q_out``, the cache) count as changed in place: autograd
+refuses a backward pass that had saved what they held, as after any such operator of torch.
 """
 from __future__ import annotations
 
@@ -23,6 +26,7 @@ from typing import Optional
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from .. import _native
 
@@ -231,6 +235,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
             raise ValueError("rotary has a gradient only without out and stream")
         _on_gpu("rotary", device)
         return _Rotary.apply(x, positions, inv_freq, (bool(interleaved), float(magnitude), 1.0))
+    given = out
     if out is None:
         _on_gpu("rotary", device)
         out = _empty_like(x, stream)
@@ -241,7 +246,11 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
             _no_gradient("rotary into out")
         _own_memory(out, "out")
         _on_gpu("rotary", device)
-    return _turn(x, positions, inv_freq, bool(interleaved), float(magnitude), 1.0, out, stream) if 0 not in shape else out
+    if 0 not in shape:
+        _turn(x, positions, inv_freq, bool(interleaved), float(magnitude), 1.0, out, stream)
+        if given is not None:
+            increment_version(given)
+    return out
 
 
 def _batch(pool, page_table, seq_lens, query_starts, device):
@@ -335,6 +344,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
     at, turn = pool.data_ptr(), pairs > 0
     groups = ((k.data_ptr(), at, 0, *k.stride(), page, token, head, element, kv_heads, turn, 0),
               (v.data_ptr(), at + plane * 2, 0, *v.stride(), page, token, head, element, kv_heads, 0, 1))
+    written = [pool]
     if q is not None:
         q_shape = _rows(q, "q", pool, dim, device)
         if q_shape[0] != rows:
@@ -346,6 +356,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
             if _rows(q_out, "q_out", pool, dim, device) != q_shape:
                 raise ValueError("q_out must have the shape of q")
             _own_memory(q_out, "q_out")
+            written.append(q_out)
         groups += ((q.data_ptr(), q_out.data_ptr(), 0, *q.stride(), 0, *q_out.stride(), q_shape[1], 1, -1),)
     elif q_out is not None:
         raise ValueError("q_out needs q")
@@ -355,6 +366,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, pool: torch.Tensor, page_tabl
                               pos64, 0, pos_stride, batch, _TYPES[pool.dtype], device, _stream(stream, device), status_ptr)
         if err:
             _check(err, "paged_append")
+        increment_version(written)
     return pool if q is None else (pool, q_out)
 
 
@@ -419,6 +431,8 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
             _TYPES[pool.dtype], device, _stream(stream, device), status_ptr)
         if err:
             _check(err, "paged_attention")
+        if not fresh:
+            increment_version(out)
     return (out, lse) if return_lse else out
 
 

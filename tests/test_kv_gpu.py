@@ -663,3 +663,30 @@ def test_attention_says_when_a_table_is_too_narrow_or_the_pool_empty(causal):
     got, bits = run(q, pool[:0], table, lens, none)
     assert bits == 4 and not got.any()
     assert run(q, pool[:0], table, lens * 0, none)[1] == 0
+
+
+def test_writes_are_seen_by_autograd():
+    """A tensor that some operator saved for its backward pass is written by ours: the backward pass says so."""
+    args, _ = _attention_case([1, 3], [20, 40], q_heads=4, kv_heads=2, dim=64, seed=42)
+    q, pool, table, lens, starts = args
+    k, v = _randn(4, 2, 64, seed=1), _randn(4, 2, 64, seed=2)
+    freq, pos = ops.rotary_frequencies(64, device="cuda"), torch.arange(4, device="cuda")
+    batch = (pool, table, lens, starts)
+    out = torch.empty_like(q)
+    for to, call in ((q, lambda: ops.rotary(q, pos, freq, out=q)), (out, lambda: ops.rotary(q, pos, freq, out=out)),
+                     (pool, lambda: ops.paged_append(k, v, *batch)),
+                     (q, lambda: ops.paged_append(k, v, *batch, inv_freq=freq, q=q, q_out=q)),
+                     (out, lambda: ops.paged_append(k, v, *batch, inv_freq=freq, q=q, q_out=out)),
+                     (out, lambda: ops.paged_attention(q, *batch, out=out)), (q, lambda: ops.paged_attention(q, *batch, out=q))):
+        w = torch.ones((), dtype=BF16, device="cuda", requires_grad=True)
+        y = (to * w).sum()  # saves `to`
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    read = (q, k, v, table, lens, starts, pos, freq)
+    was = [t._version for t in read]
+    ops.rotary(q, pos, freq), ops.paged_append(k, v, *batch, inv_freq=freq, q=q), ops.paged_attention(q, *batch)
+    assert [t._version for t in read] == was
+    with torch.inference_mode():
+        x = torch.zeros(4, 2, 64, dtype=BF16, device="cuda")
+        ops.rotary(x, pos, freq, out=x)
