@@ -125,7 +125,7 @@ struct PagedAttentionArgs {
     float scale = 1.f;
     int causal = 1;
     int64_t window = 0;  // keys that a causal row sees, itself among them; 0: all
-    int fill_tail = 0;   // write zeros (lse -inf) to rows behind the last sequence
+    int fill_tail = 0;   // write zeros to rows of no sequence (their lse is -inf in any case)
     KvBatch batch;
     void *workspace = nullptr;
     size_t workspace_bytes = 0;

@@ -369,10 +369,10 @@ struct Kernel {
         if (gave_up() && lane == 0)
             for (int s = 0; s < 2; ++s)
                 if (n_q[s]) mbar_wait_bounded(&c->q_full[s], (n_q[s] - 1) & 1, g.budget / 8);
-        if (g.a.fill_tail) fill_tail();
+        if (g.a.fill_tail || g.a.lse) fill_tail();
     }
 
-    // Zeros in the rows of no sequence.
+    // The rows of no sequence: zeros in an output that is to have them, -inf in log-sum-exps.
     __device__ void fill_tail() const {
         const PagedAttentionArgs &a = g.a;
         const int n = a.batch.seqs;
@@ -381,7 +381,7 @@ struct Kernel {
         const int64_t rows = head + a.rows - tail, per = a.q_heads * static_cast<int64_t>(a.dim);
         for (int64_t i = blockIdx.x * 32 + lane; i < rows * per; i += gridDim.x * 32) {
             const int64_t k = i / per, e = i - k * per, row = k < head ? k : tail + (k - head);
-            static_cast<T *>(a.out)[row * a.o_st + e / a.dim * a.o_sh + e % a.dim] = from_f32<T>(0.f);
+            if (a.fill_tail) static_cast<T *>(a.out)[row * a.o_st + e / a.dim * a.o_sh + e % a.dim] = from_f32<T>(0.f);
             if (a.lse && e % a.dim == 0) a.lse[row * a.q_heads + e / a.dim] = -INFINITY;
         }
     }

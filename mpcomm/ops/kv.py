@@ -383,11 +383,11 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
 
     Returns the output in ``out`` (its padding rows stay as they were) or in a new tensor (zeros there), with
     ``return_lse`` also the rows' log-sum-exp of the scaled scores, fp32 ``[tokens, q_heads]``, by which results over
-    parts of a context can be joined. A row that sees no key gives zeros and -inf. Keys on pages that the table or
-    the pool does not have (a table too narrow for ``seq_lens`` among them) are not seen, and set bit 2 of the uint32
-    device word at ``status_ptr``. Slots behind a
-    sequence's end or before its window may hold anything, NaN included; a NaN or infinity in a value that some new
-    token sees may reach the other new tokens of its sequence.
+    parts of a context can be joined. A row that sees no key gives zeros and -inf, a padding row -inf.
+    Keys on pages that the table or the pool does not have (a table too narrow for ``seq_lens`` among them) are not
+    seen, and set bit 2 of the uint32 device word at ``status_ptr``. Slots behind a sequence's end or before its
+    window may hold anything, NaN included; a NaN or infinity in a value that some new token sees may reach the other
+    new tokens of its sequence.
 
     bf16 and fp16, ``head_dim`` a multiple of 8 up to 128, ``page_tokens`` a multiple of 8, all strides of ``q``,
     ``out`` and ``pool`` multiples of 16 bytes but the last, which is one element. The cache is in device memory.

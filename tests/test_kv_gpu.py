@@ -690,3 +690,15 @@ def test_writes_are_seen_by_autograd():
     with torch.inference_mode():
         x = torch.zeros(4, 2, 64, dtype=BF16, device="cuda")
         ops.rotary(x, pos, freq, out=x)
+
+
+def test_attention_fills_the_log_sum_exp_of_padding_rows():
+    """-inf whether the output is new or given."""
+    args, _ = _attention_case([1, 3], [200, 40], dim=64, pad=70, seed=41)
+    q, pool, table, lens, starts = args
+    starts = starts + 2  # padding in front, too
+    for out in (None, torch.empty_like(q)):
+        junk = torch.full(q.shape[:2], 5.0, device="cuda")
+        del junk
+        lse = ops.paged_attention(q, pool, table, lens, starts, out=out, return_lse=True)[1]
+        assert (lse[:2] == -math.inf).all() and (lse[6:] == -math.inf).all() and lse[2:6].isfinite().all()
