@@ -702,3 +702,25 @@ def test_attention_fills_the_log_sum_exp_of_padding_rows():
         del junk
         lse = ops.paged_attention(q, pool, table, lens, starts, out=out, return_lse=True)[1]
         assert (lse[:2] == -math.inf).all() and (lse[6:] == -math.inf).all() and lse[2:6].isfinite().all()
+
+
+@pytest.mark.parametrize("dim,q_heads", [(8, 1), (24, 5), (64, 40), (72, 3), (96, 7), (128, 32)])
+@pytest.mark.parametrize("front,behind", [(0, 700), (300, 0), (5, 1), (700, 300)])
+def test_attention_of_batches_that_are_mostly_padding(dim, q_heads, front, behind):
+    """Rows of no sequence before and behind the batch's: zeros and -inf, and nothing else is touched."""
+    args, _ = _attention_case([1, 3], [200, 40], q_heads, 1, dim, pad=front + behind, dtype=FP16, seed=43)
+    q, pool, table, lens, starts = args
+    starts = starts + front
+    want, want_lse, tol, ltol = ref.attention(q, pool, table, lens, starts)
+    live = slice(front, front + 4)
+    junk = torch.full(q.shape, 5.0, dtype=FP16, device="cuda")
+    del junk
+    got, lse = ops.paged_attention(q, pool, table, lens, starts, return_lse=True)
+    _near(got[live], want[live], tol[live])
+    _near(lse[live], want_lse[live], ltol[live])
+    for rows in (slice(0, front), slice(front + 4, None)):
+        assert not got[rows].any() and (lse[rows] == -math.inf).all()
+    out = torch.full((q.shape[0], q_heads + 1, dim), 7.0, dtype=FP16, device="cuda")
+    ops.paged_attention(q, pool, table, lens, starts, out=out[:, :q_heads])
+    assert torch.equal(out[live, :q_heads], got[live]) and (out[:, q_heads] == 7.0).all()
+    assert (out[:front] == 7.0).all() and (out[front + 4:] == 7.0).all()
