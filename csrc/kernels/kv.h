@@ -133,7 +133,14 @@ struct PagedAttentionArgs {
 };
 // Bytes of workspace that a call needs (its contents do not matter), 16-byte aligned.
 size_t paged_attention_workspace(int dim, int device);
+// A wait in the kernel that runs out (wait_budget_ns(); never in a run that
+// works) sets kStatusLoadTimeout in `status` and ends the call with outputs
+// that mean nothing. Without `status` the next call on any device returns
+// kWaitRanOut, once, and does nothing.
+constexpr int kWaitRanOut = -1;
 int paged_attention(const PagedAttentionArgs &a, int dtype, int device, void *stream);
+// Says on the host what a kernel says whose wait ran out (for tests). False without a GPU.
+bool paged_attention_give_up();
 
 }  // namespace kern
 }  // namespace mpcomm

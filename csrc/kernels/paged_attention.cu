@@ -48,6 +48,7 @@
 // runs for seconds).
 #include <atomic>
 #include <cstring>
+#include <mutex>
 
 #include "cuda/gpu.h"
 #include "kernels/attention_plan.h"
@@ -148,6 +149,7 @@ struct KernelArgs {
     int ctas;
     int box;  // tokens of a full box
     int box_shift;  // a block has 2^box_shift boxes
+    uint32_t *gave_up;  // host memory: where a kernel without a status word says that a wait ran out
     uint64_t budget;  // of a wait, ns
     uint32_t tries;   // the same, in tries of a microsecond
 };
@@ -173,6 +175,11 @@ struct Kernel {
 
     __device__ uint32_t *status() const { return g.a.status ? g.a.status : &g_attention_status; }
 
+    __device__ __noinline__ void ran_out() const {
+        if (g.a.status) atomicOr(g.a.status, kStatusLoadTimeout);
+        else *static_cast<volatile uint32_t *>(g.gave_up) = 1;
+    }
+
     // Waits for a phase; gives up after the budget (a try waits for about a microsecond), and at once when any wait
     // of the CTA has given up.
     __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity) const {
@@ -182,7 +189,7 @@ struct Kernel {
             if (*dead) break;
             if (--left == 0) {
                 *dead = 1;
-                atomicOr(status(), kStatusLoadTimeout);
+                ran_out();
             }
         }
     }
@@ -595,7 +602,7 @@ struct Kernel {
         // are done.
         if (elect_one()) {
             mma_commit(&c->drain[s]);
-            mbar_wait_bounded(&c->drain[s], 0, g.budget);
+            if (!mbar_wait_bounded(&c->drain[s], 0, g.budget)) ran_out();
         }
         __syncwarp();
     }
@@ -992,6 +999,27 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     }
 }
 
+// A word of pinned host memory that kernels write whose wait ran out, and that
+// the next call reads: such a kernel ends with outputs that mean nothing, and
+// no call waits for the GPU to see it. Null where there is no GPU.
+uint32_t *gave_up_word() {
+    static std::mutex mu;
+    static std::atomic<uint32_t *> word{nullptr};
+    if (uint32_t *w = word.load(std::memory_order_acquire)) return w;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!word.load(std::memory_order_relaxed)) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // the first call may be a captured one
+        void *p = nullptr;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+        const cudaError_t e = cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) return nullptr;
+        std::memset(p, 0, 64);
+        word.store(static_cast<uint32_t *>(p), std::memory_order_release);
+    }
+    return word.load(std::memory_order_relaxed);
+}
+
 // CTAs that a call is given: no more than its units can be, and one an SM.
 int plan_ctas(const PagedAttentionArgs &a, const PlanShape &s, int sms) {
     const int64_t blocks = s.tokens > kBlockKeys ? (s.tokens + kBlockKeys - 1) / kBlockKeys : 1;
@@ -1109,6 +1137,12 @@ size_t paged_attention_workspace(int dim, int device) {
     return shared_bytes(sms) + 2 * static_cast<size_t>(sms) * slot_bytes(dim <= 64 ? 64 : 128);
 }
 
+bool paged_attention_give_up() {
+    uint32_t *word = gave_up_word();
+    if (word) __atomic_store_n(word, 1u, __ATOMIC_RELEASE);
+    return word != nullptr;
+}
+
 int paged_attention(const PagedAttentionArgs &a, int dtype, int device, void *stream) {
     if (a.rows <= 0 || a.q_heads <= 0) return 0;
     if (a.dim <= 0 || a.dim % 8 || a.dim > 128 || a.kv_heads <= 0 || a.q_heads % a.kv_heads || a.rows > 0x7fffffff ||
@@ -1118,6 +1152,9 @@ int paged_attention(const PagedAttentionArgs &a, int dtype, int device, void *st
     if (on.error()) return on.error();
     KernelArgs g;
     g.a = a;
+    g.gave_up = gave_up_word();
+    if (!g.gave_up) return cudaErrorMemoryAllocation;
+    if (*static_cast<volatile uint32_t *>(g.gave_up) && __atomic_exchange_n(g.gave_up, 0u, __ATOMIC_ACQ_REL)) return kWaitRanOut;
     const int64_t tokens = a.batch.pages > 0 ? a.batch.table_width * a.batch.page_tokens : 0;
     g.group = a.q_heads / a.kv_heads;
     plan_parts(&g.shape, a.kv_heads, g.group);

@@ -34,6 +34,7 @@ __all__ = ["rotary_frequencies", "rotary", "paged_append", "paged_attention"]
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _CACHE_TYPES = (torch.bfloat16, torch.float16)
+_WAIT_RAN_OUT = -1  # of a native call
 _INDEX = {torch.int32: 0, torch.int64: 1}
 
 
@@ -389,6 +390,9 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
     window may hold anything, NaN included; a NaN or infinity in a value that some new token sees may reach the other
     new tokens of its sequence.
 
+    The kernel's waits are bounded. One that ran out (a GPU that does not work as it should) leaves outputs that mean
+    nothing: it sets bit 0 of the word at ``status_ptr``, and without one the next call raises a ``RuntimeError``.
+
     bf16 and fp16, ``head_dim`` a multiple of 8 up to 128, ``page_tokens`` a multiple of 8, all strides of ``q``,
     ``out`` and ``pool`` multiples of 16 bytes but the last, which is one element. The cache is in device memory.
     """
@@ -430,6 +434,9 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
             dim ** -0.5 if scale is None else float(scale), bool(causal), window, fresh, batch, space.data_ptr(), need,
             _TYPES[pool.dtype], device, _stream(stream, device), status_ptr)
         if err:
+            if err == _WAIT_RAN_OUT:
+                raise RuntimeError("mpcomm paged_attention: a wait in an earlier call's kernel ran out, what that call "
+                                   "returned is not to be used; this call did nothing")
             _check(err, "paged_attention")
         if not fresh:
             increment_version(out)

@@ -969,6 +969,9 @@ PYBIND11_MODULE(_mpcomm, m) {
         py::arg("workspace"), py::arg("workspace_bytes"), py::arg("dtype"), py::arg("device"), py::arg("stream"),
         py::arg("status") = 0);
 
+    m.def("_paged_attention_give_up", &kern::paged_attention_give_up,
+          "Marks, on the host, that a wait of a paged_attention kernel ran out (tests).");
+
     // ---- host-side fault hooks of the loopback fabric (tests) ----
     m.def("_lo_inject_wc_errors", &fabric::loopback_inject_wc_errors, py::arg("gid"), py::arg("count"));
     m.def("_lo_set_port_active", &fabric::loopback_set_port_active, py::arg("gid"), py::arg("active"));

@@ -1,5 +1,8 @@
 """GPU tests of rotary positions, appending to a paged KV cache and attention over it, against 64-bit forms."""
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -8,7 +11,7 @@ import kv_reference as ref
 
 pytestmark = pytest.mark.gpu
 
-from mpcomm import ops  # noqa: E402
+from mpcomm import _native, ops  # noqa: E402
 from mpcomm.models import KVPoolSpec  # noqa: E402
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
@@ -724,3 +727,40 @@ def test_attention_of_batches_that_are_mostly_padding(dim, q_heads, front, behin
     ops.paged_attention(q, pool, table, lens, starts, out=out[:, :q_heads])
     assert torch.equal(out[live, :q_heads], got[live]) and (out[:, q_heads] == 7.0).all()
     assert (out[:front] == 7.0).all() and (out[front + 4:] == 7.0).all()
+
+
+def test_attention_says_that_a_wait_of_an_earlier_call_ran_out():
+    """The word that such a kernel writes is written from the host here: the next call raises, the one after works."""
+    args, _ = _attention_case([1, 3], [200, 40], dim=64, seed=44)
+    want = ops.paged_attention(*args)
+    for out in (None, torch.zeros_like(args[0])):
+        assert _native._paged_attention_give_up()
+        with pytest.raises(RuntimeError, match="a wait in an earlier call's kernel ran out"):
+            ops.paged_attention(*args, out=out)
+        assert out is None or not out.any()
+        assert torch.equal(ops.paged_attention(*args, out=out), want)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.paged_attention(*args, status_ptr=status.data_ptr())
+    assert status.item() == 0
+
+
+def test_attention_whose_first_call_is_captured():
+    """In a process of its own: what the first call sets up is set up while a stream is being captured."""
+    code = """
+import torch
+import kv_reference as ref
+from mpcomm import ops
+table, lens, starts, pages = ref.batch([1, 3], [200, 40], 16, device="cuda")
+pool, q = (torch.randn(s, device="cuda").bfloat16() for s in ((pages, 2, 2, 16, 64), (4, 8, 64)))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = ops.paged_attention(q, pool, table, lens, starts)
+graph.replay()
+want, _, tol, _ = ref.attention(q, pool, table, lens, starts)
+assert ((out.double() - want).abs() <= tol).all()
+assert torch.equal(ops.paged_attention(q, pool, table, lens, starts), out)
+"""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join((here, os.path.dirname(here))))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0, r.stderr[-2000:]
