@@ -1,6 +1,8 @@
 """Paged KV cache operators without a GPU: frequencies, cache views and every refusal."""
 import math
 import os
+import re
+import shutil
 import subprocess
 import sys
 import types
@@ -331,3 +333,24 @@ def test_no_silent_loss_of_tangents():
             kv._Rotary.backward(saved, dual(x))
         _refused(lambda: ops.rotary(x, pos, freq), for_the_device=True)  # plain tensors are taken
         _refused(lambda: _call("attention"), for_the_device=True)
+
+
+def test_attention_kernels_have_the_registers_that_their_warps_divide(tmp_path):
+    """The warps take and give registers of what a CTA is launched with, which is what the compiler chose: as many as
+    the source counts on, or every launch is refused. Nothing may be spilled either."""
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("no CUDA compiler")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    source = os.path.join(root, "csrc", "kernels", "paged_attention.cu")
+    want = re.search(r"kRegsLaunch = (\d+)", open(source).read()).group(1)
+    r = subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-DNDEBUG", "--expt-relaxed-constexpr",
+                        "-std=c++17", "-I" + os.path.join(root, "csrc"), "-I" + os.path.join(root, "include"), "-Xptxas", "-v",
+                        "-cubin", "-o", str(tmp_path / "kernels.cubin"), source], capture_output=True, text=True, timeout=500)
+    assert r.returncode == 0, r.stderr[-2000:]
+    found = re.findall(r"Compiling entry function '\S*?(paged_attention_kernel|join_kernel)(?:.*\n)*?.*?(\d+) bytes spill stores"
+                       r"(?:.*\n)*?.*?Used (\d+) registers", r.stderr)
+    assert sorted(name for name, _, _ in found) == ["join_kernel"] * 4 + ["paged_attention_kernel"] * 4, r.stderr[-2000:]
+    for name, spilled, registers in found:
+        assert spilled == "0"
+        assert name == "join_kernel" or registers == want
