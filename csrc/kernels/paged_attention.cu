@@ -524,7 +524,11 @@ struct Kernel {
             const int n = 2 * (pair ? r.blocks : (r.blocks + 1 - s) / 2);  // half blocks
             // With the same rows in both streams, blocks 2 t and 2 t + 1 are taken together, one by each stream.
             const bool before = !pair && s == 1;
-            const bool early = pair || (L::kKeys >= 4 && r.blocks >= 16);
+            // Scores of the next block before this one's values are free: always for two streams of rows, and for one
+            // where K has four tiles (heads of up to 64; single tokens of 64 sequences of 8,192 take 258 us, later 281;
+            // of 256 of 500, 114 and 119). With two tiles the streams hold both, and little is left to load ahead: 256
+            // of 500 would take 132 us for 134, but 64 of 8,192 would take 357 for 352.
+            const bool early = pair || L::kKeys >= 4;
             wait(&c->q_full[0], n_q[0]++ & 1);
             if (pair && s == 1) wait(&c->q_full[1], n_q[1]++ & 1);
             tmem_fence_after();
@@ -587,8 +591,6 @@ struct Kernel {
                 if (early) {
                     if (i + 2 < n) scores(i + 2);
                 } else if ((i & 1) && i + 1 < n) {
-                    // K of a stream's next block only after V of this one is free: with few tiles in the rings the two
-                    // streams would hold four, and there would be little room to load ahead
                     scores(i + 1);
                     scores(i + 2);
                 }
