@@ -764,3 +764,10 @@ assert torch.equal(ops.paged_attention(q, pool, table, lens, starts), out)
     env = dict(os.environ, PYTHONPATH=os.pathsep.join((here, os.path.dirname(here))))
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, env=env)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_attention_counts_tiles_of_long_prompts():
+    """Sequences of 15 to 33 tiles of 64 tokens, whose tiles a lane or a warp counts, among single tokens."""
+    news = [960, 1, 1024, 1025, 1, 2117]
+    args, how = _attention_case(news, [960, 300, 1500, 1025, 1, 2200], q_heads=4, kv_heads=1, dim=64, spoil=True, seed=45)
+    _check_attention(args, how, news)
