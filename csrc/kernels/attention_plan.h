@@ -4,9 +4,12 @@
 // fit into kStreamRows, token by token, and a tile is two streams' tokens. A
 // tile reads the blocks of kBlockKeys keys that some row of it sees. The unit
 // of work is one block of one tile. All units stand in one line (sequence,
-// part, tile, block); every CTA takes an equal, contiguous share of it, so
-// the work is even whatever the lengths are, and neighbours read the same
-// keys.
+// part, tile, block); every CTA takes a contiguous share of equally many
+// units, so neighbours read the same keys. A unit is a block whatever its tile
+// is: shares are even in blocks for any lengths, and in time where all tiles
+// have one stream's rows or all have two's. In a batch of both, the CTAs with
+// the tiles of two streams end last (about 2 us a block; two chunks of 512
+// tokens take 90 us, 32 single tokens 82, both together 165).
 #ifndef MPCOMM_B200_CSRC_KERNELS_ATTENTION_PLAN_H_
 #define MPCOMM_B200_CSRC_KERNELS_ATTENTION_PLAN_H_
 

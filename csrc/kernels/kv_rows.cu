@@ -133,8 +133,9 @@ struct RowsShape {
 // then a lane of the block's (row, head) pairs. A thread holds its first
 // pair's elements before the rows' places, sines and cosines are known, and
 // always those of the next pair while it turns and stores one, so that the
-// trips to memory overlap (two pairs ahead: 3 % slower). A block's sines and cosines are computed once for
-// all heads. N > 1 needs unit element strides, 16-byte aligned bases and
+// trips to memory overlap (two pairs ahead, in registers, at the price of
+// occupancy: 3 % slower). A block's sines and cosines are computed once for all
+// heads. N > 1 needs unit element strides, 16-byte aligned bases and
 // strides and pairs, dim multiples of N (of N / 2 for interleaved pairs).
 template <typename T, int N, bool INTERLEAVED, bool PAGED>
 __global__ void __launch_bounds__(kRowThreads, 4) kv_rows_kernel(const __grid_constant__ KvRowsArgs a, const __grid_constant__ RowsShape g) {

@@ -25,10 +25,11 @@
 //   warp 11         loads the queries and V blocks
 //
 // Weights are rounded to the cache's type for the second product, whose two
-// operands have one type; sums, maxima, scores and outputs are 32-bit. m only
-// moves when a score passes the one it was taken from by 2^8 (kRescale), so
-// O_s is hardly ever rescaled. In bf16 m is that score and weights reach 2^8.
-// In fp16 weights below 2^-14 have a step of 2^-24, so m is taken 2^7 lower
+// operands have one type (outputs in bf16 are off by 0.0023 of their norm, by
+// 0.0017 through their own rounding alone); sums, maxima, scores and outputs
+// are 32-bit. m only moves when a score passes the one it was taken from by
+// 2^8 (kRescale), so O_s is hardly ever rescaled. In bf16 m is that score and
+// weights reach 2^8. In fp16 weights below 2^-14 have a step of 2^-24, so m is taken 2^7 lower
 // (kDepth): weights reach 2^15 of the 65,504 that the type holds, and each is
 // off by at most 2^-25 where the largest is at least 2^7, 2^-32 of it. (With m
 // at the score, 8,191 keys 25.2 powers of two below one other lost half of
@@ -43,9 +44,9 @@
 // MB: 97 us, 5.5 TB/s; the products are done for 128 rows, most of them
 // unused, and keep the tensor pipe busy for a third of that). Chunks, the chain
 // of a half block's scores, exponentials and products, of which two overlap:
-// 1,024 tokens over 8,192 take 133 us (969 TFLOP/s), 4,096 over 16,384 take
-// 808 (1.19 PFLOP/s; a library product reaches 1.66 in a burst, 1.38 when it
-// runs for seconds).
+// 1,024 tokens over 8,192 take 133 us (971 TFLOP/s), 4,096 over 16,384 take
+// 798 alone, after a pause (1.21 PFLOP/s), and 932 back to back (1.03; a
+// library product reaches 1.66 in a burst, 1.38 when it runs for seconds).
 #include <atomic>
 #include <cstring>
 #include <mutex>
@@ -623,7 +624,7 @@ struct Kernel {
     // Replaces, in tensor memory, a half block's scores of columns outside [lo, hi) and on boxes that are not there;
     // its first column is key `at` of its block. Few blocks need it, so it is little code away from the loop's:
     // fetching instructions that run once a tile is what costs here. A way through them on registers, with a copy of
-    // the loop's step, took 3 us a tile more (windows of 512 tokens, 8 x 777 new tokens: 99 us, this 85).
+    // the loop's step, took 3 us a tile more (windows of 512 tokens, 8 x 777 new tokens, cold: 99 us, with this 85, now 82).
     __device__ __forceinline__ void mask_scores(uint32_t ts, int lo, int hi, int at, uint32_t boxes) const {
         const int shift = 7 - g.box_shift;
 #pragma unroll 1

@@ -214,7 +214,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     ``positions`` has the shape of its token axes, or ``[tokens]`` for all of a batch (int32 or int64, negative ones
     turn back). Of each head the first ``2 * len(inv_freq)`` elements are turned, the pairs being elements ``i`` and
     ``i + len(inv_freq)``, or ``2 i`` and ``2 i + 1`` with ``interleaved``; the rest is copied unscaled. Angles are
-    reduced in 64 bits, so positions may be as far as they like.
+    reduced in 64 bits, off by at most 2^-51 of themselves: by 2^-20 radians at a position of 2^31 and a radian each.
 
     ``out`` may be ``x`` itself, or memory apart from it. Differentiable in ``x`` (any number of times) without
     ``out`` and ``stream``, not in ``inv_freq``: frequencies that require a gradient are refused, and so is
