@@ -11,8 +11,9 @@ import kv_reference as ref
 
 pytestmark = pytest.mark.gpu
 
-from mpcomm import _native, ops  # noqa: E402
+from mpcomm import ops  # noqa: E402
 from mpcomm.models import KVPoolSpec  # noqa: E402
+from mpcomm import _native  # noqa: E402
 
 BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
 
