@@ -395,6 +395,7 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, page_table: torch.Tenso
 
     bf16 and fp16, ``head_dim`` a multiple of 8 up to 128, ``page_tokens`` a multiple of 8, all strides of ``q``,
     ``out`` and ``pool`` multiples of 16 bytes but the last, which is one element. The cache is in device memory.
+    A call takes a workspace of its own, 39 MB on 148 SMs for heads over 64 and 20 MB up to 64, whatever its sizes.
     """
     device = q.get_device()
     cache, batch = _batch(pool, page_table, seq_lens, query_starts, device)
